@@ -51,6 +51,7 @@ typedef enum ms_qtype {
   MS_Q_Q8_0 = 8,
   MS_Q_Q4_K = 12,
   MS_Q_Q6_K = 14,
+  MS_Q_BF16 = 30,              /* element type of the attention operators only */
   MS_Q_MXFP4 = 39
 } ms_qtype;
 
@@ -235,6 +236,119 @@ MS_API int ms_model_batch_kernels_per_step(const ms_model* m);
 /* device microseconds per batch step of each launch class alone (step start, QKV, attention, O,
  * router, expert grouping, gate_up, down, residual, LM head) */
 MS_API ms_status ms_model_batch_profile_step(ms_model* m, float* us, int max, int* n);
+
+/* ---- attention operators of ragged batches: queries / keys prepared in one pass, prompt attention,
+ *      and attention over a K/V cache held in 4 bits ----
+ * No counterpart in the reference, whose cache is f32 and whose batch shares one position
+ * (model/kv_cache.rs:37-60).  All of them
+ *   - run on the context's device and stream, allocate nothing and can be captured into a graph; a
+ *     caller that has work on the tensors in another stream orders the two streams itself;
+ *   - check sizes, strides and types on the host (MS_ERR_INVALID_ARG: a pointer is missing;
+ *     MS_ERR_SHAPE: a size, stride or alignment; MS_ERR_UNSUPPORTED_QTYPE: a type) before anything
+ *     is launched, also when ctx is NULL (a dry run of the checks that ends in MS_ERR_INVALID_ARG);
+ *   - check what only the device knows (positions, lengths, page numbers) in the kernel: a bad entry
+ *     is skipped and raises MS_ERR_DEVICE_INDEX at the next ms_sync;
+ *   - take element types MS_Q_F16 and MS_Q_BF16 (MS_Q_F32 where stated) and strides in elements
+ *     between tokens; the heads of one token are contiguous. */
+
+/* Per-head RMSNorm of q and k (x / sqrt(mean(x^2) + eps) * w; no norm when both weights are NULL) and
+ * RoPE of the first rot_dim dims of every head with the row pos[t] of the tables, computed in f32 and
+ * rounded once to out_type.  Pairs: (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved.
+ * in_type / out_type: f32, f16 or bf16.  An output may be its own input (same pointer, stride and type),
+ * and must not overlap the inputs otherwise.  A token whose position is outside [0, max_pos) is not
+ * written.  head_dim even and <= 512; n_tokens may be 0. */
+typedef struct ms_qk_rope {
+  int n_tokens, heads, kv_heads, head_dim, rot_dim, interleaved;
+  int in_type, out_type;
+  float eps;
+  int max_pos;                 /* rows of the tables */
+  const void *q, *k;           /* [n_tokens][heads / kv_heads][head_dim] */
+  int64_t q_stride, k_stride;
+  const float *q_norm, *k_norm;     /* [head_dim], both or neither */
+  const float *cos_t, *sin_t;  /* [max_pos][rot_dim / 2] */
+  const int32_t* pos;          /* [n_tokens] */
+  void *q_out, *k_out;
+  int64_t q_out_stride, k_out_stride;
+} ms_qk_rope;
+MS_API ms_status ms_qk_norm_rope(ms_ctx* ctx, const ms_qk_rope* args);
+
+/* Causal attention of n_seqs packed sequences: queries cu_q[i] .. cu_q[i + 1] (rows of q and out) over
+ * keys cu_k[i] .. cu_k[i + 1] (rows of k and v); the last query stands at the last key, so a sequence
+ * with more keys than queries continues a cached prefix.  Query at key index p attends keys j <= p, and
+ * j > p - window when window > 0; sinks [heads] (f32, or NULL) join the softmax denominator.
+ * out = softmax(scale q k^T) v in f32 with the probabilities rounded to the element type for the second
+ * product; a query without keys gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.
+ * total_q / total_k: rows of q and out / of k and v (cu_q[n_seqs] and cu_k[n_seqs] at most).
+ * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 128 per kv head; strides multiples of
+ * 8 elements, pointers 16-byte aligned; out must not overlap the inputs.  The values of v are finite. */
+typedef struct ms_prompt_attn {
+  int n_seqs, heads, kv_heads, head_dim, type, window;
+  int total_q, total_k;
+  float scale;                 /* 0: 1 / sqrt(head_dim) */
+  const void *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  const int32_t *cu_q, *cu_k;  /* [n_seqs + 1], ascending from 0 (device) */
+  const float* sinks;
+  void* out;
+  int64_t out_stride;
+} ms_prompt_attn;
+MS_API ms_status ms_prompt_attention(ms_ctx* ctx, const ms_prompt_attn* args);
+
+/* A paged K/V cache in 4 bits: pages [n_pages][kv_heads][page_tokens / 16] blocks of 16 tokens and
+ * 20 * head_dim bytes; block_table[i][j] is the page of tokens [j * page_tokens, (j + 1) * page_tokens)
+ * of sequence i (entries of pages that a call does not touch may be anything).  With G = head_dim / 32
+ * groups of 32 dims, a code c in 0..15 stands for o + d * (16 + c), d and o in f16 per token and group
+ * (d = (max - min) / 15, o = min - 16 d; values clamped to +-16384, NaN becomes 0).  Inside a block:
+ *   K codes  u32 [16 tokens][4 t][G w]: dim 32 w + 8 t + 2 n + h at bits 4 n + 16 h;
+ *   K scales f16 [16 tokens][G][d, o];
+ *   V codes  u16 [8 token pairs][head_dim / 16 chunks][4 i][2 tokens]: dim 16 C + 4 i + n of chunk C at
+ *            bits 4 n, chunk C of pair p stored at C ^ ((p & 3) << 1) (at C ^ (p & 2) when head_dim is 64);
+ *   V scales f16 [8 token pairs][G][d of both tokens, o of both tokens].
+ * (The codes sit as the tensor-core fragments of ms_kv4_attention want them.)  head_dim 64, 128 or 256;
+ * page_tokens a power of two in 16 .. 1024; pages 16-byte aligned. */
+typedef struct ms_kv4_cache {
+  int kv_heads, head_dim, page_tokens, n_pages;
+  void* pages;
+  const int32_t* block_table;  /* [n_seqs][max_pages] (device) */
+  int n_seqs, max_pages;
+} ms_kv4_cache;
+/* bytes of one page (all heads, K and V) */
+MS_API ms_status ms_kv4_page_bytes(int kv_heads, int head_dim, int page_tokens, size_t* bytes);
+
+/* Quantise packed rows k / v [total][kv_heads][head_dim] (f32, f16 or bf16) into the cache, or read the
+ * cache back into them (rounded once from f32): rows cu[i] .. cu[i + 1] are the tokens start[i],
+ * start[i] + 1, ... of sequence i.  Rows behind cu[n_seqs] are skipped.  Writing touches the bytes of its own
+ * tokens only; two calls that write the same token at the same time leave either. */
+typedef struct ms_kv4_rows {
+  int type, total;
+  const int32_t *cu, *start;   /* [n_seqs + 1] ascending from 0, [n_seqs] (device) */
+  void *k, *v;
+  int64_t k_stride, v_stride;
+} ms_kv4_rows;
+MS_API ms_status ms_kv4_write(ms_ctx* ctx, const ms_kv4_cache* cache, const ms_kv4_rows* rows);
+MS_API ms_status ms_kv4_read(ms_ctx* ctx, const ms_kv4_cache* cache, const ms_kv4_rows* rows);
+
+/* Attention of the newest n_query tokens of every sequence over its cache (their own K/V already
+ * written): sequence i holds lens[i] tokens, query t of n_query stands at token lens[i] - n_query + t and
+ * attends tokens j <= that, j > that - window when window > 0; sinks [heads] or NULL.  A query without
+ * tokens (lens[i] = 0) gives zeros.  q / out [n_seqs][n_query][heads][head_dim], contiguous, f16 or bf16;
+ * scores from the exact codes in f32, probabilities and dequantised V rounded to f16 for the second
+ * product (f32 accumulation).  heads a multiple of kv_heads; n_query * heads / kv_heads <= 128.
+ * work: ms_kv4_attention_workspace bytes (16-byte aligned) that this call alone uses while it runs: calls
+ * (or captured graphs) that may overlap need one each. */
+typedef struct ms_kv4_attn {
+  int n_query, heads, type, window;
+  float scale;                 /* 0: 1 / sqrt(head_dim) */
+  const void* q;
+  const int32_t* lens;         /* [n_seqs] (device) */
+  const float* sinks;
+  void* out;
+  void* work;
+  size_t work_bytes;
+} ms_kv4_attn;
+MS_API ms_status ms_kv4_attention_workspace(const ms_ctx* ctx, const ms_kv4_cache* cache, int n_query, int heads,
+                                            size_t* bytes);
+MS_API ms_status ms_kv4_attention(ms_ctx* ctx, const ms_kv4_cache* cache, const ms_kv4_attn* args);
 
 /* ---- hybrid (Qwen3.5 / Qwen3-Next) blocks ---- */
 /* One Gated DeltaNet layer in device memory.  Projections are in native blocks (qtype as in

@@ -10,7 +10,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # the CUDA binding is imported lazily so GGUF tooling works without the built library
-    if name in ("Context", "Engine", "config_from_model"):
+    if name in ("Context", "Engine", "KV4Cache", "config_from_model"):
         from . import engine
         return getattr(engine, name)
     raise AttributeError(name)

@@ -56,6 +56,44 @@ class DeltaNetLayer(C.Structure):
                 ("conv1d", C.c_void_p), ("ssm_a", C.c_void_p), ("dt_bias", C.c_void_p), ("norm", C.c_void_p)]
 
 
+class QkRope(C.Structure):
+    """ms_qk_rope: per-head norm and rotation of queries and keys (device pointers as ints)."""
+    _fields_ = [("n_tokens", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("rot_dim", C.c_int), ("interleaved", C.c_int), ("in_type", C.c_int), ("out_type", C.c_int),
+                ("eps", C.c_float), ("max_pos", C.c_int), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("pos", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_out", C.c_void_p), ("q_out_stride", C.c_int64), ("k_out_stride", C.c_int64)]
+
+
+class PromptAttn(C.Structure):
+    """ms_prompt_attn: causal attention of packed sequences (device pointers as ints)."""
+    _fields_ = [("n_seqs", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("type", C.c_int), ("window", C.c_int), ("total_q", C.c_int), ("total_k", C.c_int),
+                ("scale", C.c_float), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("cu_q", C.c_void_p),
+                ("cu_k", C.c_void_p), ("sinks", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
+class Kv4CacheArgs(C.Structure):
+    """ms_kv4_cache: the paged 4-bit K/V cache (device pointers as ints)."""
+    _fields_ = [("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int), ("n_pages", C.c_int),
+                ("pages", C.c_void_p), ("block_table", C.c_void_p), ("n_seqs", C.c_int), ("max_pages", C.c_int)]
+
+
+class Kv4Rows(C.Structure):
+    """ms_kv4_rows: packed K/V rows written into or read from the cache (device pointers as ints)."""
+    _fields_ = [("type", C.c_int), ("total", C.c_int), ("cu", C.c_void_p), ("start", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64)]
+
+
+class Kv4Attn(C.Structure):
+    """ms_kv4_attn: attention of each sequence's newest tokens over the cache (device pointers as ints)."""
+    _fields_ = [("n_query", C.c_int), ("heads", C.c_int), ("type", C.c_int), ("window", C.c_int),
+                ("scale", C.c_float), ("q", C.c_void_p), ("lens", C.c_void_p), ("sinks", C.c_void_p),
+                ("out", C.c_void_p), ("work", C.c_void_p), ("work_bytes", C.c_size_t)]
+
+
 _lib = None
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
 _ip = C.POINTER(C.c_int32)
@@ -110,6 +148,13 @@ _SIGS = {
     "ms_model_router_stats": (C.c_int, [_vp, _fp, _ip]),
     "ms_model_router_totals": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i, C.POINTER(C.c_int)]),
     "ms_model_expert_tier_stats": (C.c_int, [_vp, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
+    "ms_qk_norm_rope": (C.c_int, [_vp, C.POINTER(QkRope)]),
+    "ms_prompt_attention": (C.c_int, [_vp, C.POINTER(PromptAttn)]),
+    "ms_kv4_page_bytes": (C.c_int, [_i, _i, _i, C.POINTER(C.c_size_t)]),
+    "ms_kv4_write": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows)]),
+    "ms_kv4_read": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows)]),
+    "ms_kv4_attention_workspace": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), _i, _i, C.POINTER(C.c_size_t)]),
+    "ms_kv4_attention": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Attn)]),
     "ms_model_get_config": (C.c_int, [_vp, C.POINTER(ModelConfig)]),
     "ms_model_destroy": (C.c_int, [_vp]),
     "ms_model_forward": (C.c_int, [_vp, _ip, _i, _fp]),

@@ -4,6 +4,12 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+struct ms_qk_rope;
+struct ms_prompt_attn;
+struct ms_kv4_cache;
+struct ms_kv4_rows;
+struct ms_kv4_attn;
+
 namespace ms {
 
 // ---- device error word bits (the host reads them through ms_ctx_error_flags) ----
@@ -498,6 +504,14 @@ cudaError_t launch_silu_mul(const float* g, const float* u, float* o, int n, cud
 // y += sigmoid(x . gate_inp) * v (assign: y = ...); gate_inp null: factor 1
 cudaError_t launch_gated_accum(const float* x, const float* gate_inp, const float* v, float* y, int n, cudaStream_t s,
                                int assign = 0);
+
+// ---- attention operators of ragged batches (arguments checked by the callers in runtime.cu) ----
+cudaError_t launch_qk_rope(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s);                    // kernels_qk_rope.cu
+cudaError_t launch_prompt_attention(const DevCtx& c, const ms_prompt_attn& a, cudaStream_t s);       // kernels_prompt_attn.cu
+cudaError_t launch_kv4_rows(const DevCtx& c, const ms_kv4_cache& kv, const ms_kv4_rows& r, bool write,
+                            cudaStream_t s);                                                         // kernels_kv4.cu
+size_t kv4_attn_workspace(const DevCtx& c, const ms_kv4_cache& kv, int n_query, int heads);          // kernels_kv4_attn.cu
+cudaError_t launch_kv4_attention(const DevCtx& c, const ms_kv4_cache& kv, const ms_kv4_attn& a, cudaStream_t s);
 
 // ---- step plumbing ----
 // ---- sampling (kernels_sample.cu): SamplingParams::sample (engine.rs:124-208) on the device ----

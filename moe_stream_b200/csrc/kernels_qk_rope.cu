@@ -1,0 +1,192 @@
+// kernels_qk_rope.cu — per-head RMSNorm of queries and keys and the position rotation, in one pass.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w   (per head; skipped without weights)
+//   (a, b) -> (a cos - b sin, b cos + a sin)   on the first rot_dim dims, pairs (i, i + rot_dim / 2) or
+//                                              (2 i, 2 i + 1), row pos[t] of the tables
+//
+// Everything is computed in f32 and rounded once to the output's type.  Bound by memory: each row is read and
+// written once.
+#include "../../include/moestream_cuda.h"
+#include "attn_types.cuh"
+#include "common.cuh"
+#include "kernels.h"
+
+namespace ms {
+namespace {
+
+constexpr int kThreads = 128;
+
+// One group of LPR = head_dim / 16 lanes holds a head: two chunks of 8 dims per lane, the two sides of its
+// rotation pairs where it rotates (dims 8 l .. and rot / 2 + 8 l ..), otherwise dims 16 l .. 16 l + 15.  A group
+// takes HPG heads of one token, whose table row and norm weights stay in registers.
+template <class TI, class TO, int LPR, int HPG, bool INTER>
+__global__ void __launch_bounds__(kThreads) qk_rope_kernel(const ms_qk_rope a, uint32_t* err) {
+  const int lane = threadIdx.x % LPR;
+  const uint32_t item = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+  const uint32_t nbq = (a.heads + HPG - 1) / HPG, nb = nbq + (a.kv_heads + HPG - 1) / HPG;
+  const uint32_t t = item / nb, hb = item % nb;
+  const bool is_q = hb < nbq;
+  const int h0 = (is_q ? hb : hb - nbq) * HPG, nh = is_q ? a.heads : a.kv_heads;
+  bool live = t < (uint32_t)a.n_tokens;
+  int pos = 0;
+  if (live) {
+    pos = a.pos[t];
+    if (pos < 0 || pos >= a.max_pos) {
+      if (hb == 0 && lane == 0) atomicOr(err, EF_BAD_INDEX);
+      live = false;
+    }
+  }
+  constexpr int HD = LPR * 16;
+  const int half = a.rot_dim / 2;
+  const bool turns = 16 * lane < a.rot_dim;
+  const int d0 = !INTER && turns ? 8 * lane : 16 * lane, d1 = !INTER && turns ? d0 + half : d0 + 8;
+  const TI* src = (const TI*)(is_q ? a.q : a.k) + (int64_t)t * (is_q ? a.q_stride : a.k_stride);
+  TO* dst = (TO*)(is_q ? a.q_out : a.k_out) + (int64_t)t * (is_q ? a.q_out_stride : a.k_out_stride);
+  Raw8<TI> r[HPG][2];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i)
+    if (live && h0 + i < nh) {
+      r[i][0].load(src + (h0 + i) * HD + d0);
+      r[i][1].load(src + (h0 + i) * HD + d1);
+    }
+  float cs[8], sn[8], w[16];
+  if (live && turns) {   // 8 pairs per lane: (8 l + i, half + 8 l + i), or 2 i and 2 i + 1 of its 16 dims
+    const float4* c4 = reinterpret_cast<const float4*>(a.cos_t + (int64_t)pos * half + 8 * lane);
+    const float4* s4 = reinterpret_cast<const float4*>(a.sin_t + (int64_t)pos * half + 8 * lane);
+    *reinterpret_cast<float4*>(cs) = c4[0]; *reinterpret_cast<float4*>(cs + 4) = c4[1];
+    *reinterpret_cast<float4*>(sn) = s4[0]; *reinterpret_cast<float4*>(sn + 4) = s4[1];
+  }
+  const float* nw = is_q ? a.q_norm : a.k_norm;
+  if (nw) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { w[i] = nw[d0 + i]; w[8 + i] = nw[d1 + i]; }
+  }
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    float x[2][8];
+    r[i][0].get(x[0]);
+    r[i][1].get(x[1]);
+    if (nw) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[0][j], x[0][j], fmaf(x[1][j], x[1][j], ss));
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { x[0][j] *= inv * w[j]; x[1][j] *= inv * w[8 + j]; }
+    }
+    if (turns) {
+      if (INTER) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float u = x[c][2 * j], v = x[c][2 * j + 1], co = cs[4 * c + j], si = sn[4 * c + j];
+            x[c][2 * j] = u * co - v * si;
+            x[c][2 * j + 1] = v * co + u * si;
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float u = x[0][j], v = x[1][j];
+          x[0][j] = u * cs[j] - v * sn[j];
+          x[1][j] = v * cs[j] + u * sn[j];
+        }
+      }
+    }
+    if (live && h0 + i < nh) {
+      store8(dst + (h0 + i) * HD + d0, x[0]);
+      store8(dst + (h0 + i) * HD + d1, x[1]);
+    }
+  }
+}
+
+// Any even head_dim up to 512, any even rot_dim, any alignment: one warp per head, through shared memory.
+template <class TI, class TO>
+__global__ void __launch_bounds__(kThreads) qk_rope_any_kernel(const ms_qk_rope a, uint32_t* err) {
+  __shared__ float sh[kThreads / 32][512];
+  const int lane = threadIdx.x & 31, hd = a.head_dim, half = a.rot_dim / 2;
+  float* x = sh[threadIdx.x >> 5];
+  const uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), nh = a.heads + a.kv_heads;
+  const uint32_t t = item / nh;
+  const int hh = item % nh;
+  if (t >= (uint32_t)a.n_tokens) return;
+  const int pos = a.pos[t];
+  if (pos < 0 || pos >= a.max_pos) {
+    if (hh == 0 && lane == 0) atomicOr(err, EF_BAD_INDEX);
+    return;
+  }
+  const bool is_q = hh < a.heads;
+  const int h = is_q ? hh : hh - a.heads;
+  const TI* src = (const TI*)(is_q ? a.q : a.k) + (int64_t)t * (is_q ? a.q_stride : a.k_stride) + h * hd;
+  TO* dst = (TO*)(is_q ? a.q_out : a.k_out) + (int64_t)t * (is_q ? a.q_out_stride : a.k_out_stride) + h * hd;
+  float ss = 0.f;
+  for (int i = lane; i < hd; i += 32) {
+    const float v = to_f32(src[i]);
+    x[i] = v;
+    ss = fmaf(v, v, ss);
+  }
+  const float* nw = is_q ? a.q_norm : a.k_norm;
+  __syncwarp();
+  if (nw) {
+    const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)hd + a.eps);
+    for (int i = lane; i < hd; i += 32) x[i] *= inv * nw[i];
+    __syncwarp();
+  }
+  for (int i = lane; i < half; i += 32) {
+    const int i0 = a.interleaved ? 2 * i : i, i1 = a.interleaved ? 2 * i + 1 : i + half;
+    const float u = x[i0], v = x[i1], c = a.cos_t[(int64_t)pos * half + i], s = a.sin_t[(int64_t)pos * half + i];
+    x[i0] = u * c - v * s;
+    x[i1] = v * c + u * s;
+  }
+  __syncwarp();
+  for (int i = lane; i < hd; i += 32) dst[i] = from_f32<TO>(x[i]);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <class TI, class TO, int LPR, int HPG>
+void start_vec(const ms_qk_rope& a, uint32_t* err, cudaStream_t s) {
+  const uint32_t nb = (a.heads + HPG - 1) / HPG + (a.kv_heads + HPG - 1) / HPG;
+  const uint32_t grid = ((uint64_t)a.n_tokens * nb + kThreads / LPR - 1) / (kThreads / LPR);
+  if (a.interleaved) qk_rope_kernel<TI, TO, LPR, HPG, true><<<grid, kThreads, 0, s>>>(a, err);
+  else qk_rope_kernel<TI, TO, LPR, HPG, false><<<grid, kThreads, 0, s>>>(a, err);
+}
+
+template <class TI, class TO>
+void start(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
+  const int hd = a.head_dim;
+  const bool vec = (hd == 64 || hd == 128 || hd == 256) && a.rot_dim % 16 == 0 && a.q_stride % 8 == 0 &&
+                   a.k_stride % 8 == 0 && a.q_out_stride % 8 == 0 && a.k_out_stride % 8 == 0 && aligned16(a.q) &&
+                   aligned16(a.k) && aligned16(a.q_out) && aligned16(a.k_out) && aligned16(a.cos_t) && aligned16(a.sin_t);
+  if (!vec) {
+    const uint64_t items = (uint64_t)a.n_tokens * (a.heads + a.kv_heads);
+    qk_rope_any_kernel<TI, TO><<<(uint32_t)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, s>>>(a, c.err);
+    return;
+  }
+  // few rows: one head per group, so that the loads of a decode step spread over the SMs
+  const bool wide = (int64_t)a.n_tokens * (a.heads + a.kv_heads) * hd / 16 >= (int64_t)c.sm_count * 4 * 2048;
+  if (hd == 64) wide ? start_vec<TI, TO, 4, 4>(a, c.err, s) : start_vec<TI, TO, 4, 1>(a, c.err, s);
+  else if (hd == 128) wide ? start_vec<TI, TO, 8, 4>(a, c.err, s) : start_vec<TI, TO, 8, 1>(a, c.err, s);
+  else wide ? start_vec<TI, TO, 16, 4>(a, c.err, s) : start_vec<TI, TO, 16, 1>(a, c.err, s);
+}
+
+template <class TI>
+void start_out(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
+  if (a.out_type == MS_Q_F32) start<TI, float>(c, a, s);
+  else if (a.out_type == MS_Q_F16) start<TI, __half>(c, a, s);
+  else start<TI, __nv_bfloat16>(c, a, s);
+}
+
+}  // namespace
+
+cudaError_t launch_qk_rope(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
+  if (a.n_tokens == 0) return cudaSuccess;
+  if (a.in_type == MS_Q_F32) start_out<float>(c, a, s);
+  else if (a.in_type == MS_Q_F16) start_out<__half>(c, a, s);
+  else start_out<__nv_bfloat16>(c, a, s);
+  return cudaGetLastError();
+}
+
+}  // namespace ms

@@ -1670,6 +1670,190 @@ ms_status ms_rope(ms_ctx* c, const float* x, const float* cs, const float* sn, i
   return MS_OK;
 }
 
+// ---- attention operators of ragged batches ----
+// Arguments are checked before anything is launched; `why` gets the reason.  A null context runs the checks only.
+namespace {
+
+bool elem_type(int t, bool f32) { return t == MS_Q_F16 || t == MS_Q_BF16 || (f32 && t == MS_Q_F32); }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// the device of the context for one call; the caller's current device comes back
+struct OnDevice {
+  int prev = -1;
+  explicit OnDevice(int device) {
+    if (cudaGetDevice(&prev) != cudaSuccess || prev == device) prev = -1;
+    else cudaSetDevice(device);
+  }
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+ms_status check_qk_rope(const ms_qk_rope& a, const char** why) {
+  if (a.n_tokens < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.max_pos <= 0)
+    return *why = "n_tokens >= 0, heads, kv_heads and max_pos > 0 required", MS_ERR_SHAPE;
+  if (a.head_dim <= 0 || a.head_dim % 2 || a.head_dim > 512 || a.rot_dim <= 0 || a.rot_dim % 2 || a.rot_dim > a.head_dim)
+    return *why = "head_dim even and <= 512, rot_dim even and <= head_dim required", MS_ERR_SHAPE;
+  if (!elem_type(a.in_type, true) || !elem_type(a.out_type, true))
+    return *why = "f32, f16 or bf16 required", MS_ERR_UNSUPPORTED_QTYPE;
+  const int64_t q = (int64_t)a.heads * a.head_dim, k = (int64_t)a.kv_heads * a.head_dim;
+  if (a.q_stride < q || a.q_out_stride < q || a.k_stride < k || a.k_out_stride < k)
+    return *why = "a stride is smaller than a token's heads", MS_ERR_SHAPE;
+  if ((int64_t)a.n_tokens * ((int64_t)a.heads + a.kv_heads) > 0x7fffff00ll) return *why = "too many rows", MS_ERR_SHAPE;
+  if (!(a.eps >= 0.0f)) return *why = "eps >= 0 required", MS_ERR_INVALID_ARG;
+  if ((a.q_norm == nullptr) != (a.k_norm == nullptr)) return *why = "q_norm and k_norm go together", MS_ERR_INVALID_ARG;
+  if (a.n_tokens && (!a.q || !a.k || !a.q_out || !a.k_out || !a.cos_t || !a.sin_t || !a.pos))
+    return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
+  if ((a.q_out == a.q && (a.q_out_stride != a.q_stride || a.in_type != a.out_type)) ||
+      (a.k_out == a.k && (a.k_out_stride != a.k_stride || a.in_type != a.out_type)))
+    if (a.n_tokens) return *why = "in place needs the input's stride and type", MS_ERR_INVALID_ARG;
+  return MS_OK;
+}
+
+ms_status check_prompt(const ms_prompt_attn& a, const char** why) {
+  if (a.n_seqs < 0 || a.total_q < 0 || a.total_k < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads)
+    return *why = "counts >= 0 and heads a multiple of kv_heads required", MS_ERR_SHAPE;
+  if (a.heads / a.kv_heads > 128) return *why = "at most 128 heads per kv head", MS_ERR_SHAPE;
+  if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return *why = "head_dim 64, 128 or 256 required", MS_ERR_SHAPE;
+  if (!elem_type(a.type, false)) return *why = "f16 or bf16 required", MS_ERR_UNSUPPORTED_QTYPE;
+  const int64_t q = (int64_t)a.heads * a.head_dim, k = (int64_t)a.kv_heads * a.head_dim;
+  if (a.q_stride < q || a.out_stride < q || a.k_stride < k || a.v_stride < k)
+    return *why = "a stride is smaller than a token's heads", MS_ERR_SHAPE;
+  if (a.q_stride % 8 || a.out_stride % 8 || a.k_stride % 8 || a.v_stride % 8)
+    return *why = "strides must be multiples of 8 elements", MS_ERR_SHAPE;
+  if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16))
+    return *why = "pointers must be 16-byte aligned", MS_ERR_SHAPE;
+  if (!std::isfinite(a.scale) || a.scale < 0.0f) return *why = "scale > 0 (or 0 for the default) required", MS_ERR_INVALID_ARG;
+  if (a.total_q && a.n_seqs && (!a.q || !a.out || !a.cu_q || !a.cu_k)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
+  if (a.total_q && a.n_seqs && a.total_k && (!a.k || !a.v)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
+  if (a.total_q && (a.out == a.q || (a.total_k && (a.out == a.k || a.out == a.v))))
+    return *why = "out must not overlap the inputs", MS_ERR_INVALID_ARG;
+  return MS_OK;
+}
+
+ms_status check_cache(const ms_kv4_cache& c, const char** why) {
+  if (c.kv_heads <= 0 || c.n_pages < 0 || c.n_seqs < 0 || c.max_pages < 0)
+    return *why = "kv_heads > 0 and counts >= 0 required", MS_ERR_SHAPE;
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return *why = "head_dim 64, 128 or 256 required", MS_ERR_SHAPE;
+  if (c.page_tokens < 16 || c.page_tokens > 1024 || (c.page_tokens & (c.page_tokens - 1)))
+    return *why = "page_tokens must be a power of two in 16 .. 1024", MS_ERR_SHAPE;
+  if ((int64_t)c.max_pages * c.page_tokens > 0x7fff0000ll) return *why = "too many tokens per sequence", MS_ERR_SHAPE;
+  if (!aligned(c.pages, 16)) return *why = "pages must be 16-byte aligned", MS_ERR_SHAPE;
+  if ((c.n_pages && !c.pages) || (c.n_seqs && c.max_pages && !c.block_table))
+    return *why = "pages or block_table missing", MS_ERR_INVALID_ARG;
+  return MS_OK;
+}
+
+ms_status check_rows(const ms_kv4_cache& c, const ms_kv4_rows& r, const char** why) {
+  const ms_status st = check_cache(c, why);
+  if (st != MS_OK) return st;
+  if (r.total < 0 || (int64_t)r.total * c.kv_heads > 0x7fffff00ll / 32) return *why = "total outside its range", MS_ERR_SHAPE;
+  if (!elem_type(r.type, true)) return *why = "f32, f16 or bf16 required", MS_ERR_UNSUPPORTED_QTYPE;
+  const int64_t k = (int64_t)c.kv_heads * c.head_dim;
+  if (r.k_stride < k || r.v_stride < k || r.k_stride % 8 || r.v_stride % 8)
+    return *why = "strides must be multiples of 8 elements and hold a token's heads", MS_ERR_SHAPE;
+  if (!aligned(r.k, 16) || !aligned(r.v, 16)) return *why = "k and v must be 16-byte aligned", MS_ERR_SHAPE;
+  if (r.total && c.n_seqs && (!r.cu || !r.start || !r.k || !r.v)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
+  return MS_OK;
+}
+
+ms_status check_kv4_shape(const ms_kv4_cache& c, int n_query, int heads, const char** why) {
+  const ms_status st = check_cache(c, why);
+  if (st != MS_OK) return st;
+  if (n_query <= 0 || heads <= 0 || heads % c.kv_heads || (int64_t)n_query * (heads / c.kv_heads) > 128)
+    return *why = "n_query > 0, heads a multiple of kv_heads, n_query * heads / kv_heads <= 128 required", MS_ERR_SHAPE;
+  if ((int64_t)c.n_seqs * n_query * heads > 0x7fffff00ll / 32 || c.n_seqs > 65535) return *why = "too many rows", MS_ERR_SHAPE;
+  return MS_OK;
+}
+
+ms_status check_kv4_attn(const ms_kv4_cache& c, const ms_kv4_attn& a, const char** why) {
+  const ms_status st = check_kv4_shape(c, a.n_query, a.heads, why);
+  if (st != MS_OK) return st;
+  if (!elem_type(a.type, false)) return *why = "f16 or bf16 required", MS_ERR_UNSUPPORTED_QTYPE;
+  if (!std::isfinite(a.scale) || a.scale < 0.0f) return *why = "scale > 0 (or 0 for the default) required", MS_ERR_INVALID_ARG;
+  if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.work, 16))
+    return *why = "pointers must be 16-byte aligned", MS_ERR_SHAPE;
+  if (c.n_seqs && (!a.q || !a.out || !a.lens || !a.work)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
+  if (c.n_seqs && a.out == a.q) return *why = "out must not overlap q", MS_ERR_INVALID_ARG;
+  return MS_OK;
+}
+
+}  // namespace
+
+ms_status ms_qk_norm_rope(ms_ctx* c, const ms_qk_rope* a) {
+  if (!a) return MS_ERR_INVALID_ARG;
+  const char* why = "";
+  const ms_status st = check_qk_rope(*a, &why);
+  if (st != MS_OK) return fail(c, st, "qk_norm_rope: %s", why);
+  if (!c) return MS_ERR_INVALID_ARG;
+  OnDevice on(c->device);
+  MS_CUDA(c, launch_qk_rope(c->dc, *a, c->stream));
+  return MS_OK;
+}
+
+ms_status ms_prompt_attention(ms_ctx* c, const ms_prompt_attn* args) {
+  if (!args) return MS_ERR_INVALID_ARG;
+  const char* why = "";
+  ms_prompt_attn a = *args;
+  const ms_status st = check_prompt(a, &why);
+  if (st != MS_OK) return fail(c, st, "prompt_attention: %s", why);
+  if (!c) return MS_ERR_INVALID_ARG;
+  if (a.scale == 0.0f) a.scale = (float)(1.0 / std::sqrt((double)a.head_dim));
+  OnDevice on(c->device);
+  MS_CUDA(c, launch_prompt_attention(c->dc, a, c->stream));
+  return MS_OK;
+}
+
+ms_status ms_kv4_page_bytes(int kv_heads, int hd, int page_tokens, size_t* bytes) {
+  if (!bytes) return MS_ERR_INVALID_ARG;
+  ms_kv4_cache c = {};
+  c.kv_heads = kv_heads; c.head_dim = hd; c.page_tokens = page_tokens;
+  const char* why = "";
+  const ms_status st = check_cache(c, &why);
+  if (st != MS_OK) return st;
+  *bytes = (size_t)kv_heads * (page_tokens / 16) * 20 * hd;
+  return MS_OK;
+}
+
+static ms_status kv4_rows(ms_ctx* c, const ms_kv4_cache* kv, const ms_kv4_rows* r, bool write) {
+  if (!kv || !r) return MS_ERR_INVALID_ARG;
+  const char* why = "";
+  const ms_status st = check_rows(*kv, *r, &why);
+  if (st != MS_OK) return fail(c, st, "kv4 %s: %s", write ? "write" : "read", why);
+  if (!c) return MS_ERR_INVALID_ARG;
+  if (!kv->n_seqs) return MS_OK;
+  OnDevice on(c->device);
+  MS_CUDA(c, launch_kv4_rows(c->dc, *kv, *r, write, c->stream));
+  return MS_OK;
+}
+ms_status ms_kv4_write(ms_ctx* c, const ms_kv4_cache* kv, const ms_kv4_rows* r) { return kv4_rows(c, kv, r, true); }
+ms_status ms_kv4_read(ms_ctx* c, const ms_kv4_cache* kv, const ms_kv4_rows* r) { return kv4_rows(c, kv, r, false); }
+
+ms_status ms_kv4_attention_workspace(const ms_ctx* c, const ms_kv4_cache* kv, int n_query, int heads, size_t* bytes) {
+  if (!kv || !bytes) return MS_ERR_INVALID_ARG;
+  const char* why = "";
+  const ms_status st = check_kv4_shape(*kv, n_query, heads, &why);
+  if (st != MS_OK) return st;
+  if (!c) return MS_ERR_INVALID_ARG;
+  *bytes = kv4_attn_workspace(c->dc, *kv, n_query, heads);
+  return MS_OK;
+}
+
+ms_status ms_kv4_attention(ms_ctx* c, const ms_kv4_cache* kv, const ms_kv4_attn* args) {
+  if (!kv || !args) return MS_ERR_INVALID_ARG;
+  const char* why = "";
+  ms_kv4_attn a = *args;
+  const ms_status st = check_kv4_attn(*kv, a, &why);
+  if (st != MS_OK) return fail(c, st, "kv4_attention: %s", why);
+  if (!c) return MS_ERR_INVALID_ARG;
+  if (a.work_bytes < kv4_attn_workspace(c->dc, *kv, a.n_query, a.heads))
+    return fail(c, MS_ERR_SHAPE, "kv4_attention: the workspace is smaller than ms_kv4_attention_workspace says");
+  if (a.scale == 0.0f) a.scale = (float)(1.0 / std::sqrt((double)kv->head_dim));
+  OnDevice on(c->device);
+  MS_CUDA(c, launch_kv4_attention(c->dc, *kv, a, c->stream));
+  return MS_OK;
+}
+
 ms_status ms_sample(ms_ctx* c, const float* logits, int V, const uint32_t* counts, float temperature, float top_p,
                     float repetition_penalty, float r, float* work, int32_t* token) {
   if (!c || !logits || !work || !token || V <= 0) return MS_ERR_INVALID_ARG;

@@ -1,0 +1,126 @@
+"""CPU checks of the attention operators: what their entry points refuse (a null context runs the checks alone),
+and the 4-bit cache's layout."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from moe_stream_b200 import _lib
+
+from . import attn_ref as R
+
+INVALID, QTYPE, SHAPE = 1, 6, 7
+P = 4096   # stands for a device pointer; nothing is launched
+
+
+@pytest.fixture(scope="module")
+def L():
+    from moe_stream_b200 import build
+    build.build()
+    return _lib.lib()
+
+
+def make(cls, **kw):
+    a = cls()
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+ROPE = dict(n_tokens=3, heads=8, kv_heads=2, head_dim=128, rot_dim=64, in_type=0, out_type=30, eps=1e-6, max_pos=10, q=P,
+            k=P, q_stride=1024, k_stride=256, q_norm=P, k_norm=P, cos_t=P, sin_t=P, pos=P, q_out=2 * P, k_out=2 * P,
+            q_out_stride=1024, k_out_stride=256)
+PROMPT = dict(n_seqs=2, heads=8, kv_heads=2, head_dim=64, type=30, total_q=10, total_k=20, q=P, k=P, v=P, q_stride=512,
+              k_stride=128, v_stride=128, cu_q=P, cu_k=P, out=2 * P, out_stride=512)
+CACHE = dict(kv_heads=2, head_dim=128, page_tokens=16, n_pages=5, pages=P, block_table=P, n_seqs=2, max_pages=3)
+ROWS = dict(type=30, total=7, cu=P, start=P, k=P, v=P, k_stride=256, v_stride=256)
+ATTN = dict(n_query=1, heads=8, type=1, q=P, lens=P, out=2 * P, work=P, work_bytes=1 << 30)
+
+
+@pytest.mark.parametrize("change,status", [
+    ({}, INVALID), (dict(n_tokens=0, q=None, pos=None), INVALID),     # fine but for the context
+    (dict(n_tokens=-1), SHAPE), (dict(heads=0), SHAPE), (dict(kv_heads=0), SHAPE), (dict(max_pos=0), SHAPE),
+    (dict(head_dim=127), SHAPE), (dict(head_dim=514, q_stride=8192, k_stride=8192), SHAPE), (dict(rot_dim=130), SHAPE),
+    (dict(rot_dim=0), SHAPE), (dict(rot_dim=7), SHAPE), (dict(in_type=8), QTYPE), (dict(out_type=2), QTYPE),
+    (dict(q_stride=1023), SHAPE), (dict(k_out_stride=255), SHAPE), (dict(n_tokens=1 << 30), SHAPE),
+    (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID), (dict(q_norm=None), INVALID), (dict(pos=None), INVALID),
+    (dict(q_out=P), INVALID),                                         # in place needs the input's type
+], ids=str)
+def test_rope_refusals(L, change, status):
+    assert L.ms_qk_norm_rope(None, C.byref(make(_lib.QkRope, **{**ROPE, **change}))) == status
+    assert L.ms_qk_norm_rope(None, None) == INVALID
+
+
+@pytest.mark.parametrize("change,status", [
+    ({}, INVALID), (dict(total_q=0, q=None, out=None), INVALID),
+    (dict(n_seqs=-1), SHAPE), (dict(total_k=-1), SHAPE), (dict(heads=9), SHAPE), (dict(heads=0), SHAPE),
+    (dict(heads=258, q_stride=1 << 15, out_stride=1 << 15), SHAPE), (dict(head_dim=96, q_stride=4096), SHAPE),
+    (dict(type=0), QTYPE), (dict(type=8), QTYPE), (dict(q_stride=504), SHAPE), (dict(v_stride=132), SHAPE),
+    (dict(k=P + 8), SHAPE), (dict(out=P + 2), SHAPE), (dict(scale=-1.0), INVALID), (dict(scale=float("inf")), INVALID),
+    (dict(cu_q=None), INVALID), (dict(v=None), INVALID), (dict(out=P), INVALID),
+], ids=str)
+def test_prompt_refusals(L, change, status):
+    assert L.ms_prompt_attention(None, C.byref(make(_lib.PromptAttn, **{**PROMPT, **change}))) == status
+
+
+CACHE_BAD = [(dict(kv_heads=0), SHAPE), (dict(head_dim=96), SHAPE), (dict(page_tokens=8), SHAPE), (dict(page_tokens=48), SHAPE),
+             (dict(page_tokens=2048), SHAPE), (dict(pages=P + 4), SHAPE), (dict(pages=None), INVALID),
+             (dict(block_table=None), INVALID), (dict(max_pages=1 << 28), SHAPE), (dict(n_seqs=-1), SHAPE)]
+
+
+@pytest.mark.parametrize("cache,rows,status", [
+    ({}, {}, INVALID), ({}, dict(total=0, k=None), INVALID),
+    *[(c, {}, s) for c, s in CACHE_BAD],
+    ({}, dict(total=-1), SHAPE), ({}, dict(total=1 << 30), SHAPE), ({}, dict(type=8), QTYPE), ({}, dict(k_stride=248), SHAPE),
+    ({}, dict(v_stride=260), SHAPE), ({}, dict(k=P + 8), SHAPE), ({}, dict(cu=None), INVALID), ({}, dict(v=None), INVALID),
+], ids=str)
+def test_cache_row_refusals(L, cache, rows, status):
+    c, r = make(_lib.Kv4CacheArgs, **{**CACHE, **cache}), make(_lib.Kv4Rows, **{**ROWS, **rows})
+    assert L.ms_kv4_write(None, C.byref(c), C.byref(r)) == status
+    assert L.ms_kv4_read(None, C.byref(c), C.byref(r)) == status
+
+
+@pytest.mark.parametrize("cache,attn,status", [
+    ({}, {}, INVALID), *[(c, {}, s) for c, s in CACHE_BAD],
+    ({}, dict(n_query=0), SHAPE), ({}, dict(heads=9), SHAPE), ({}, dict(n_query=33), SHAPE), ({}, dict(type=0), QTYPE),
+    (dict(n_seqs=70000), {}, SHAPE),
+    ({}, dict(scale=float("nan")), INVALID), ({}, dict(q=P + 2), SHAPE), ({}, dict(work=P + 8), SHAPE),
+    ({}, dict(lens=None), INVALID), ({}, dict(work=None), INVALID), ({}, dict(out=P), INVALID),
+], ids=str)
+def test_cached_attention_refusals(L, cache, attn, status):
+    c, a = make(_lib.Kv4CacheArgs, **{**CACHE, **cache}), make(_lib.Kv4Attn, **{**ATTN, **attn})
+    assert L.ms_kv4_attention(None, C.byref(c), C.byref(a)) == status
+
+
+def test_page_bytes(L):
+    n = C.c_size_t()
+    for kv, hd, page in ((1, 64, 16), (4, 128, 64), (2, 256, 1024)):
+        assert L.ms_kv4_page_bytes(kv, hd, page, C.byref(n)) == 0
+        assert n.value == kv * page // 16 * R.block_bytes(hd) == kv * page * hd * 5 // 4
+    for kv, hd, page in ((0, 64, 16), (1, 32, 16), (1, 64, 17)):
+        assert L.ms_kv4_page_bytes(kv, hd, page, C.byref(n)) == SHAPE
+    assert L.ms_kv4_page_bytes(1, 64, 16, None) == INVALID
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_layout_covers_a_block_once(hd):
+    """Every code has a nibble and every scale its bytes; together they fill the block."""
+    seen = np.zeros(R.block_bytes(hd) * 2, np.int64)             # nibbles
+    for tok in range(16):
+        for dim in range(hd):
+            for at, second in ((R._k_at, 2), (R._v_at, 4)):
+                byte, sh, sc = at(hd, tok, dim)
+                seen[2 * byte + sh // 4] += 1
+                if dim % 32 == 0:
+                    seen[2 * sc:2 * sc + 4] += 1
+                    seen[2 * (sc + second):2 * (sc + second) + 4] += 1
+    assert (seen == 1).all()
+
+
+def test_quantised_values_are_near(hd=128):
+    r = np.random.default_rng(0)
+    x = (r.standard_normal((64, 32)) * r.uniform(0.01, 50, (64, 1))).astype(np.float32)
+    c, d, o = R.quantise(x)
+    d, o = d.astype(np.float64)[:, None], o.astype(np.float64)[:, None]
+    err = np.abs(o + d * (16 + c) - x)
+    assert (err <= d * (0.5 + 31 * 2.0 ** -11) + np.abs(o) * 2.0 ** -11).all()
