@@ -7,17 +7,19 @@
 //
 // Work.  A job is (sequence, kv head, row tile); its keys are cut into tiles of TT = 4096 / head_dim tokens (5 KB).
 // The tiles of all jobs form one list that is cut into equal ranges, one per block, so sequences of any
-// lengths fill the GPU without the host knowing them.  The 4 warps of a block take the tiles of a range in
+// lengths fill the GPU without the host knowing them; each job adds kExtra empty tiles to the list, the time that
+// a block spends on the queries and the join of a job.  The 4 warps of a block take the tiles of a range in
 // turn, each with its own ring of two stages filled by bulk copies, its own running maximum and sum; they are
 // joined at the end of a job's part.  A job inside one range is finished there; the others leave their
 // numerators and sums in the workspace, which a second kernel joins.
 //
 // Scores (keys x rows, m16n8k16 in f16).  The rows of q are scaled by a power of two to a largest value in [1, 2),
 // which makes bf16 rows exact in f16 but for dims below 2^-14 of the largest (off by 2^-25 of it).  A code becomes
-// 16 + c or 256 + c by a mask-and-or after one shift for two of them; with the accumulator starting at
-// -240 (sum of the q of the 256 + c dims) the product of a group of 32 dims is P = sum q (16 + c) in f32, and
-//   s += d P + o Q,  Q = sum q
-// in f32.  Values: v = fma(16 + c, d, o) in f16 pairs of two keys, the probabilities in f16 (bf16 would
+// 16 + c or 256 + c by a mask-and-or after one shift for two of them.  With P = sum q x over a group of 32 dims as
+// the tensor core adds it, Q = sum q and R = -240 times the sum of the q of the 256 + c dims,
+//   s = sum over the groups of (d R + o Q) + d P.
+// The first part is one more product of the stored (d, o) pairs with R and Q, each cut into two f16 (22 bits);
+// the second is one f32 multiply-add a group.  Values: v = fma(16 + c, d, o) in f16 pairs of two keys, the probabilities in f16 (bf16 would
 // cost 8 times their rounding) transposed by movmatrix from the score layout.  The running maximum is raised
 // only when the probabilities of a tile grow beyond 2^8: p stays far inside f16, and most tiles need no
 // reduction over the lanes.
@@ -35,6 +37,7 @@ constexpr int kTileBytes = 5120;          // 16 * 20 * 16 for every head_dim
 // blocks of an SM: 4 leave 128 registers a thread; 256 dims, or 16 rows, need more than that
 __host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return hd * nt >= 256 ? 2 : nt == 2 ? 3 : 4; }
 constexpr int kMinTiles = kWarps;         // tiles of a range at least: one per warp
+constexpr int kExtra = 4;                 // empty tiles behind those of a job
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;           // the running maximum before any key
 constexpr float kRaise = 256.0f;          // sum of a lane's probabilities of a tile that raises the maximum
@@ -42,7 +45,7 @@ constexpr float kRaise = 256.0f;          // sum of a lane's probabilities of a 
 // ---- the list of tiles ----
 struct Plan {
   int jobs;          // of one sequence: kv heads x row tiles
-  int64_t total;     // tiles of all jobs
+  int64_t total;     // tiles of all jobs, the empty ones counted
   int64_t chunk;     // tiles of one block's range
 };
 struct SeqTiles {
@@ -50,6 +53,7 @@ struct SeqTiles {
   int lo;            // first key of any query
   int first;         // index of the first tile
   int n;             // tiles of one job, at least 1 (a sequence without tokens still gets its zeros)
+  __device__ __forceinline__ int units() const { return n + kExtra; }
 };
 template <int TT>
 __device__ __forceinline__ SeqTiles seq_tiles(const ms_kv4_cache& c, const ms_kv4_attn& a, int seq) {
@@ -68,7 +72,7 @@ __device__ __forceinline__ Plan make_plan(const ms_kv4_cache& c, const ms_kv4_at
   const int lane = threadIdx.x & 31;
   int64_t all = 0, front = 0;
   for (int i = lane; i < c.n_seqs; i += 32) {
-    const int n = seq_tiles<TT>(c, a, i).n;
+    const int n = seq_tiles<TT>(c, a, i).units();
     all += n;
     if (i < before) front += n;
   }
@@ -87,7 +91,7 @@ __device__ __forceinline__ Plan make_plan(const ms_kv4_cache& c, const ms_kv4_at
 
 // a tile of the list; every lane of a warp holds the same one
 struct Cursor {
-  int seq, job, tile;   // tile counts from s.first
+  int seq, job, tile;   // tile counts from s.first; from s.n on it is empty
   SeqTiles s;
 };
 template <int TT>
@@ -96,7 +100,7 @@ __device__ __forceinline__ Cursor find_tile(const ms_kv4_cache& c, const ms_kv4_
   Cursor k;
   int64_t at = 0;
   for (int b = 0; b < c.n_seqs; b += 32) {
-    const int64_t n = b + lane < c.n_seqs ? (int64_t)seq_tiles<TT>(c, a, b + lane).n * p.jobs : 0;
+    const int64_t n = b + lane < c.n_seqs ? (int64_t)seq_tiles<TT>(c, a, b + lane).units() * p.jobs : 0;
     int64_t inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -109,8 +113,8 @@ __device__ __forceinline__ Cursor find_tile(const ms_kv4_cache& c, const ms_kv4_
       const int64_t in = u - at - __shfl_sync(0xffffffffu, inc - n, l);
       k.seq = b + l;
       k.s = seq_tiles<TT>(c, a, k.seq);
-      k.job = (int)(in / k.s.n);
-      k.tile = (int)(in - (int64_t)k.job * k.s.n);
+      k.job = (int)(in / k.s.units());
+      k.tile = (int)(in - (int64_t)k.job * k.s.units());
       return k;
     }
     at += __shfl_sync(0xffffffffu, inc, 31);
@@ -120,8 +124,8 @@ __device__ __forceinline__ Cursor find_tile(const ms_kv4_cache& c, const ms_kv4_
 template <int TT>
 __device__ __forceinline__ void advance(const ms_kv4_cache& c, const ms_kv4_attn& a, int jobs, Cursor& k, int n) {
   k.tile += n;
-  while (k.tile >= k.s.n) {
-    k.tile -= k.s.n;
+  while (k.tile >= k.s.units()) {
+    k.tile -= k.s.units();
     if (++k.job == jobs) {
       k.job = 0;
       if (++k.seq == c.n_seqs) return;   // behind the list
@@ -141,17 +145,34 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
+// K = 8: A rows g and g + 8, k = 2 t and 2 t + 1
+__device__ __forceinline__ void mma_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
 __device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   mma(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
 }
 // the four pairs of a word (nibbles at bits 4 n and 4 n + 16) as f16 numbers: pairs 0 and 2 as 256 + c, pairs 1
 // and 3 as 16 + c, the code in the mantissa bits that weigh 1 to 8
-__device__ __forceinline__ void codes(uint32_t w, uint32_t (&x)[4]) {
+// (a three-input logic instruction takes one constant: the other two stay in registers)
+struct Bases {
+  uint32_t b256 = 0x5C005C00u, b16 = 0x4C004C00u;
+  __device__ __forceinline__ Bases() { asm volatile("" : "+r"(b256), "+r"(b16)); }
+};
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t base) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(MASK), "r"(base));
+  return r;
+}
+__device__ __forceinline__ void codes(uint32_t w, const Bases& k, uint32_t (&x)[4]) {
   const uint32_t lo = w << 2, hi = w >> 6;
-  x[0] = (lo & 0x003C003Cu) | 0x5C005C00u;
-  x[1] = (lo & 0x03C003C0u) | 0x4C004C00u;
-  x[2] = (hi & 0x003C003Cu) | 0x5C005C00u;
-  x[3] = (hi & 0x03C003C0u) | 0x4C004C00u;
+  x[0] = mask_or<0x003C003Cu>(lo, k.b256);
+  x[1] = mask_or<0x03C003C0u>(lo, k.b16);
+  x[2] = mask_or<0x003C003Cu>(hi, k.b256);
+  x[3] = mask_or<0x03C003C0u>(hi, k.b16);
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -189,8 +210,10 @@ template <int HD, int NT>
 struct Rows {
   static constexpr int G = HD / 32, MT = HD / 16;
   uint32_t q[NT][G][4];    // lane (g, t): dims 32 w + 8 t .. + 7 of row g
-  float qs[NT][G][2];      // of rows 2 t and 2 t + 1: the sum of a group's q
-  float start[NT][G][2];   // and -240 times that of its 256 + c dims
+  // (R, Q) of row g as pairs: group 4 j + t in corr[j][0] and what f16 left of it in [1]; with 2 groups, lanes
+  // t = 0, 1 hold the groups and t = 2, 3 the rests
+  static constexpr int CORR = (G + 3) / 4;
+  uint32_t corr[NT][CORR][2];
   float c2[NT][2];         // log2(e) scale times the row's power of two
   int last[NT][2];         // the row's last key (-1: no such row)
   float o[NT][MT][4], m[NT][2], l[NT][2];
@@ -198,7 +221,8 @@ struct Rows {
 
 // one tile: scores, probabilities, value product.  MASKED: some keys are not every row's
 template <int HD, int NT, bool MASKED>
-__device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const uint8_t* tile, int key0, int len, int window, uint32_t have) {
+__device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const Bases& K, const uint8_t* tile, int key0, int len, int window,
+                                          uint32_t have) {
   constexpr int G = HD / 32, TB = 256 / HD, BLK = 20 * HD, MT = HD / 16;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   // scores: s[b][n] = {key g: rows 2 t, 2 t + 1; key g + 8: the same rows}
@@ -223,26 +247,36 @@ __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const uint8_t* tile, 
         *reinterpret_cast<uint4*>(s1 + w) = *reinterpret_cast<const uint4*>(ks + 8 * G + w);
       }
     }
+    if (G == 2) {
+      const uint32_t a0 = ks[(t & 1)], a1 = ks[8 * G + (t & 1)];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) mma_k8(s[b][n], a0, a1, R.corr[n][0][0]);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[b][n][e] = 0.f;
+      for (int j = 0; j < G / 4; ++j) {
+        const uint32_t a0 = ks[4 * j + t], a1 = ks[8 * G + 4 * j + t];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (j == 0) mma(s[b][n], a0, a1, a0, a1, R.corr[n][j][0], R.corr[n][j][1], 0.f, 0.f, 0.f, 0.f);
+          else mma_add(s[b][n], a0, a1, a0, a1, R.corr[n][j][0], R.corr[n][j][1]);
+        }
+      }
+    }
 #pragma unroll
     for (int w = 0; w < G; ++w) {
       uint32_t x0[4], x1[4];
-      codes(k0[w], x0);
-      codes(k1[w], x1);
-      const float2 d0 = unpack2<__half>(s0[w]), d1 = unpack2<__half>(s1[w]);
+      codes(k0[w], K, x0);
+      codes(k1[w], K, x1);
+      const float d0 = h2f_bits((uint16_t)s0[w]), d1 = h2f_bits((uint16_t)s1[w]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float p[4];
-        mma(p, x0[0], x1[0], x0[1], x1[1], R.q[n][w][0], R.q[n][w][1], R.start[n][w][0], R.start[n][w][1], R.start[n][w][0],
-            R.start[n][w][1]);
+        mma(p, x0[0], x1[0], x0[1], x1[1], R.q[n][w][0], R.q[n][w][1], 0.f, 0.f, 0.f, 0.f);
         mma_add(p, x0[2], x1[2], x0[3], x1[3], R.q[n][w][2], R.q[n][w][3]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[b][n][i] = fmaf(d0.x, p[i], fmaf(d0.y, R.qs[n][w][i], s[b][n][i]));
-          s[b][n][2 + i] = fmaf(d1.x, p[2 + i], fmaf(d1.y, R.qs[n][w][i], s[b][n][2 + i]));
+          s[b][n][i] = fmaf(d0, p[i], s[b][n][i]);
+          s[b][n][2 + i] = fmaf(d1, p[2 + i], s[b][n][2 + i]);
         }
       }
     }
@@ -320,8 +354,8 @@ __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const uint8_t* tile, 
 #pragma unroll
       for (int i = 0; i < words; ++i) {
         uint32_t x0[4], x1[4];
-        codes(w0[i], x0);
-        codes(w1[i], x1);
+        codes(w0[i], K, x0);
+        codes(w1[i], K, x1);
         const uint32_t a0 = hfma2(minus240(x0[0]), sc0.x, sc0.y), a1 = hfma2(x0[1], sc0.x, sc0.y);
         const uint32_t a2 = hfma2(minus240(x1[0]), sc1.x, sc1.y), a3 = hfma2(x1[1], sc1.x, sc1.y);
         const uint32_t a4 = hfma2(minus240(x0[2]), sc0.x, sc0.y), a5 = hfma2(x0[3], sc0.x, sc0.y);
@@ -377,55 +411,61 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
   const int window = a.window > 0 ? a.window : 0x7fffffff;
 
   Cursor cur = find_tile<TT>(c, a, plan, u0), pre = cur;
-  // ---- the ring: tiles warp, warp + kWarps, ... of the range ----
-  auto fetch = [&](int stage) {
+  // ---- the ring: tiles warp, warp + kWarps, ... of the range; `page` is looked up one tile ahead ----
+  const bool one_page = (1 << shift) >= TT;                  // a tile lies inside one page (else lane p brings page p of it)
+  auto look_up = [&]() {
+    const int token = (pre.s.first + pre.tile) * TT + (one_page ? 0 : lane << shift);
+    const bool want = lane < (one_page ? 1 : TT >> shift) && token < pre.s.len && token + c.page_tokens > pre.s.lo;
+    return want ? c.block_table[(int64_t)pre.seq * c.max_pages + (token >> shift)] : -2;   // -2: not needed
+  };
+  auto fetch = [&](int stage, int page) {
     const int head = row_tiles > 1 ? pre.job / row_tiles : pre.job;
-    const int first = (pre.s.first + pre.tile) * TT;         // the tile's first token
-    int page = -1, n_blk = TB, blk0 = 0;                     // blocks that a lane copies, from that block of its page
-    bool want = false;
-    unsigned mask;
-    if ((1 << shift) >= TT) {                                // the tile lies inside one page
-      blk0 = (first & (c.page_tokens - 1)) >> 4;
-      want = lane == 0 && first < pre.s.len;
-    } else {                                                 // lane p brings page p of the tile
-      n_blk = 1 << (shift - 4);
-      const int token = first + (lane << shift);
-      want = lane < (TT >> shift) && token < pre.s.len && token + c.page_tokens > pre.s.lo;
-    }
-    if (want) page = c.block_table[(int64_t)pre.seq * c.max_pages + (first >> shift) + lane];
-    const bool ok = page >= 0 && page < c.n_pages;
-    if (want && !ok) atomicOr(err, EF_BAD_INDEX);
-    mask = __ballot_sync(0xffffffffu, ok);
+    const bool ok = (unsigned)page < (unsigned)c.n_pages;
+    if (page != -2 && !ok) atomicOr(err, EF_BAD_INDEX);
+    const int n_blk = one_page ? TB : 1 << (shift - 4);      // blocks that a lane copies
+    uint32_t have = ok ? ((1u << n_blk) - 1) << (one_page ? 0 : lane * n_blk) : 0u;
+    if (!one_page) have = __reduce_or_sync(0xffffffffu, have);
     if (lane == 0) {
-      uint32_t have = 0;
-#pragma unroll
-      for (int p = 0; p < TB; ++p)                           // at most TB pages
-        if (mask >> p & 1) have |= ((1u << n_blk) - 1) << (p * n_blk);
       sm.have[warp][stage] = have;
-      mbar_expect_tx(&sm.full[warp][stage], __popc(mask) * n_blk * BLK);
+      mbar_expect_tx(&sm.full[warp][stage], __popc(have) * BLK);
     }
-    __syncwarp();
+    if (!one_page) __syncwarp();
     if (ok) {
+      const int blk0 = one_page ? (((pre.s.first + pre.tile) * TT) & (c.page_tokens - 1)) >> 4 : 0;
       const int64_t blk = (((int64_t)page * c.kv_heads + head) << (shift - 4)) + blk0;
       bulk_g2s(sm.stage[warp][stage] + lane * n_blk * BLK, (const uint8_t*)c.pages + blk * BLK, n_blk * BLK, &sm.full[warp][stage]);
     }
   };
-  int next = warp, used = 0;                                 // next tile to fetch; tiles taken by this warp
-  advance<TT>(c, a, plan.jobs, pre, warp);
-  for (int i = 0; i < kStages && next < count; ++i) {
-    fetch(i);
+  int next = warp, used = 0, page = -2;                      // next tile to fetch; tiles taken by this warp
+  auto step_next = [&](int n) {                              // to the warp's next tile that is not empty
+    do {
+      advance<TT>(c, a, plan.jobs, pre, n);
+      n = kWarps;
+    } while (next < count && pre.tile >= pre.s.n && (next += kWarps) < count);
+    if (next < count) page = look_up();
+  };
+  auto fetch_next = [&](int stage) {
+    fetch(stage, page);
     next += kWarps;
-    advance<TT>(c, a, plan.jobs, pre, kWarps);
-  }
+    step_next(kWarps);
+  };
+  step_next(warp);
+  for (int i = 0; i < kStages && next < count; ++i) fetch_next(i);
 
   int at = 0;                                                // begin of the current job's part
   while (at < count) {
     const int head = row_tiles > 1 ? cur.job / row_tiles : cur.job, row0 = (cur.job - head * row_tiles) * ROWS;
-    const int end = min(count, at + cur.s.n - cur.tile);
+    const int end = min(count, at + cur.s.n - cur.tile), rest = min(count, at + cur.s.units() - cur.tile);
+    if (end <= at) {                                         // only empty tiles
+      advance<TT>(c, a, plan.jobs, cur, rest - at);
+      at = rest;
+      continue;
+    }
     const bool begins = cur.tile == 0, done = begins && end - at == cur.s.n;
     const int len = cur.s.len;
     if (threadIdx.x == 0 && begins && cur.job == 0 && a.lens[cur.seq] != len) atomicOr(err, EF_BAD_INDEX);
 
+    const Bases K;
     Rows<HD, NT> R;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -454,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
 #pragma unroll
       for (int w = 0; w < G; ++w) {
         const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
-        float s[2] = {0.f, 0.f};
+        float s[2] = {0.f, 0.f};                             // of the 256 + c and of the 16 + c dims
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float2 f = unpack2<T>(u[i]);
@@ -467,11 +507,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
           s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
           s[i] += __shfl_xor_sync(0xffffffffu, s[i], 2);
         }
-        const float all = s[0] + s[1], st = -240.f * s[0];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          R.qs[n][w][i] = __shfl_sync(0xffffffffu, all, 8 * t + 4 * i);
-          R.start[n][w][i] = __shfl_sync(0xffffffffu, st, 8 * t + 4 * i);
+        const float rr = -240.f * s[0], qq = s[0] + s[1];
+        const uint32_t whole = pack2<__half>(rr, qq);
+        const float2 f = unpack2<__half>(whole);
+        const uint32_t rest = pack2<__half>(rr - f.x, qq - f.y);
+        if (G == 2) {
+          if (w == 0 || (t & 1)) R.corr[n][0][0] = t < 2 ? whole : rest;
+        } else if (t == (w & 3)) {
+          R.corr[n][w / 4][0] = whole;
+          R.corr[n][w / 4][1] = rest;
         }
       }
 #pragma unroll
@@ -491,22 +535,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     const int t_first = row0 / rep, t_last = min(rows - 1, row0 + ROWS - 1) / rep;
     const int hi_all = len - a.n_query + t_first, lo_all = a.window > 0 ? len - a.n_query + t_last - a.window + 1 : 0;
 
-    for (int x = warp + used * kWarps; x < end; x += kWarps) {
+    for (int x = at + ((warp - at) & (kWarps - 1)); x < end; x += kWarps) {
       const int stage = used % kStages;
       const bool landed = mbar_wait(&sm.full[warp][stage], (used / kStages) & 1, err, EF_TIMEOUT_FULL);
       const uint32_t have = landed ? sm.have[warp][stage] : 0u;
       const int key0 = (cur.s.first + cur.tile + x - at) * TT;
       if (key0 >= lo_all && key0 + TT - 1 <= hi_all && have == (1u << TB) - 1)
-        take_tile<HD, NT, false>(R, sm.stage[warp][stage], key0, len, window, have);
+        take_tile<HD, NT, false>(R, K, sm.stage[warp][stage], key0, len, window, have);
       else
-        take_tile<HD, NT, true>(R, sm.stage[warp][stage], key0, len, window, have);
+        take_tile<HD, NT, true>(R, K, sm.stage[warp][stage], key0, len, window, have);
       ++used;
       __syncwarp();                                          // the stage is free
-      if (next < count) {
-        fetch(stage);
-        next += kWarps;
-        advance<TT>(c, a, plan.jobs, pre, kWarps);
-      }
+      if (next < count) fetch_next(stage);
     }
 
     // ---- join the warps: all on the largest maximum, warps 2 and 3 into 0 and 1, those through shared memory ----
@@ -585,8 +625,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
       }
     }
     __syncthreads();                                         // the buffers may be written again
-    advance<TT>(c, a, plan.jobs, cur, end - at);
-    at = end;
+    advance<TT>(c, a, plan.jobs, cur, rest - at);
+    at = rest;
   }
 }
 
@@ -600,7 +640,8 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const ms_kv4_cache c
   const int rep = a.heads / c.kv_heads, rr = (job % row_tiles) * ROWS + r;
   int64_t base;
   const Plan plan = make_plan<TT>(c, a, row_tiles, ranges, seq, &base);
-  const int64_t n = seq_tiles<TT>(c, a, seq).n, j0 = base + job * n, j1 = j0 + n;
+  const SeqTiles st = seq_tiles<TT>(c, a, seq);
+  const int64_t j0 = base + (int64_t)job * st.units(), j1 = j0 + st.n;
   const int64_t c0 = j0 / plan.chunk, c1 = (j1 - 1) / plan.chunk;
   pdl_wait_prior();                        // every block waits: this grid must not end before the first one
   if (c0 == c1 || rr >= a.n_query * rep) return;   // finished by its block, or no such row
