@@ -37,7 +37,7 @@ constexpr int kTileBytes = 5120;          // 16 * 20 * 16 for every head_dim
 // blocks of an SM: 4 leave 128 registers a thread; 256 dims, or 16 rows, need more than that
 __host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return hd * nt >= 256 ? 2 : nt == 2 ? 3 : 4; }
 constexpr int kMinTiles = kWarps;         // tiles of a range at least: one per warp
-constexpr int kExtra = 4;                 // empty tiles behind those of a job
+constexpr int kExtra = 8;                 // empty tiles behind those of a job
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;           // the running maximum before any key
 constexpr float kRaise = 256.0f;          // sum of a lane's probabilities of a tile that raises the maximum
@@ -635,7 +635,7 @@ template <class T, int HD, int NT>
 __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const ms_kv4_cache c, const ms_kv4_attn a, int row_tiles, int ranges) {
   constexpr int TT = 4096 / HD, ROWS = 8 * NT, COLS = HD / 4, GROUPS = kThreads / COLS;
   __shared__ float4 acc[kThreads];
-  __shared__ float ls[GROUPS];
+  __shared__ float ls[GROUPS], ms[GROUPS];
   const int jobs = c.kv_heads * row_tiles, seq = blockIdx.x / jobs, job = blockIdx.x % jobs, r = blockIdx.y;
   const int rep = a.heads / c.kv_heads, rr = (job % row_tiles) * ROWS + r;
   int64_t base;
@@ -647,32 +647,56 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const ms_kv4_cache c
   if (c0 == c1 || rr >= a.n_query * rep) return;   // finished by its block, or no such row
   const int h = (job / row_tiles) * rep + rr % rep;
   auto part = [&](int64_t b) { return (const float*)a.work + (b * 2 + (b == c0 ? 1 : 0)) * partial_floats<HD, ROWS>(); };
-  // the maximum first, so that the join is one sum in a fixed order
-  float top = kNone;
-  for (int64_t b = c0 + (threadIdx.x & 31); b <= c1; b += 32) top = fmaxf(top, part(b)[ROWS * HD + r]);
-  top = warp_max(top);
-  const float m = a.sinks ? fmaxf(top, a.sinks[h] * kLog2e) : top;
+  // a group of threads joins every GROUPS-th part on its own running maximum, kFlight loads under way at a time
+  constexpr int kFlight = 8;
   const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  for (int64_t b = c0 + grp; b <= c1; b += GROUPS) {
-    const float* p = part(b);
-    const float f = exp2_fast(p[ROWS * HD + r] - m);
-    const float4 x = *reinterpret_cast<const float4*>(p + r * HD + 4 * col);
-    v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
-    l += f * p[ROWS * HD + ROWS + r];
+  float m = kNone, l = 0.f;
+  for (int64_t b0 = c0 + grp; b0 <= c1; b0 += GROUPS * kFlight) {
+    float4 x[kFlight];
+    float pm[kFlight], pl[kFlight], top = m;
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int64_t b = b0 + i * GROUPS;
+      pm[i] = kNone;
+      pl[i] = 0.f;
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (b <= c1) {
+        const float* p = part(b);
+        pm[i] = p[ROWS * HD + r];
+        pl[i] = p[ROWS * HD + ROWS + r];
+        x[i] = *reinterpret_cast<const float4*>(p + r * HD + 4 * col);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) top = fmaxf(top, pm[i]);
+    float f = exp2_fast(m - top);
+    v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+    l *= f;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      f = exp2_fast(pm[i] - top);
+      v.x += f * x[i].x; v.y += f * x[i].y; v.z += f * x[i].z; v.w += f * x[i].w;
+      l += f * pl[i];
+    }
   }
   acc[threadIdx.x] = v;
-  if (col == 0) ls[grp] = l;
+  if (col == 0) { ls[grp] = l; ms[grp] = m; }
   __syncthreads();
   if (grp) return;
-  l = a.sinks ? exp2_fast(a.sinks[h] * kLog2e - m) : 0.f;
+  const float sink = a.sinks ? a.sinks[h] * kLog2e : kNone;
+  float top = sink;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, ms[i]);
+  l = a.sinks ? exp2_fast(sink - top) : 0.f;
   v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i) {
     const float4 x = acc[i * COLS + col];
-    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-    l += ls[i];
+    const float f = exp2_fast(ms[i] - top);
+    v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
+    l += f * ls[i];
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   T* dst = (T*)a.out + (((int64_t)seq * a.n_query + rr / rep) * a.heads + h) * HD + 4 * col;
