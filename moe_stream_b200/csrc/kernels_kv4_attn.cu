@@ -34,8 +34,10 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kStages = 2;
 constexpr int kTileBytes = 5120;          // 16 * 20 * 16 for every head_dim
-// blocks of an SM: 4 leave 128 registers a thread; 256 dims, or 16 rows, need more than that
-__host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return hd * nt >= 256 ? 2 : nt == 2 ? 3 : 4; }
+// blocks of an SM: 3 leave 168 registers a thread; 256 dims, or 16 rows of 128, need more than that.  (4 blocks, with
+// a few values spilled, have more warps but more starts, joins and parts: 47 us for 3's 44 on a batch of 32
+// sequences of 8,300 tokens on average, 4 heads of 128 dims.)
+__host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return hd * nt >= 256 ? 2 : 3; }
 constexpr int kMinTiles = kWarps;         // tiles of a range at least: one per warp
 constexpr int kExtra = 8;                 // empty tiles behind those of a job
 constexpr float kLog2e = 1.4426950408889634f;
@@ -43,10 +45,10 @@ constexpr float kNone = -1e30f;           // the running maximum before any key
 constexpr float kRaise = 256.0f;          // sum of a lane's probabilities of a tile that raises the maximum
 
 // ---- the list of tiles ----
-struct Plan {
+struct Plan {        // (the callers check that all tiles of a cache's capacity are below 2^31)
   int jobs;          // of one sequence: kv heads x row tiles
-  int64_t total;     // tiles of all jobs, the empty ones counted
-  int64_t chunk;     // tiles of one block's range
+  int total;         // tiles of all jobs, the empty ones counted
+  int chunk;         // tiles of one block's range
 };
 struct SeqTiles {
   int len;           // tokens (checked)
@@ -68,23 +70,20 @@ __device__ __forceinline__ SeqTiles seq_tiles(const ms_kv4_cache& c, const ms_kv
 // whole warp: the plan, and the tiles of the jobs of the sequences in front of `before`
 template <int TT>
 __device__ __forceinline__ Plan make_plan(const ms_kv4_cache& c, const ms_kv4_attn& a, int row_tiles, int ranges, int before,
-                                          int64_t* in_front) {
+                                          int* in_front) {
   const int lane = threadIdx.x & 31;
-  int64_t all = 0, front = 0;
+  int all = 0, front = 0;
   for (int i = lane; i < c.n_seqs; i += 32) {
     const int n = seq_tiles<TT>(c, a, i).units();
     all += n;
     if (i < before) front += n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    front += __shfl_xor_sync(0xffffffffu, front, o);
-  }
+  all = __reduce_add_sync(0xffffffffu, all);
+  front = __reduce_add_sync(0xffffffffu, front);
   Plan p;
   p.jobs = c.kv_heads * row_tiles;
   p.total = all * p.jobs;
-  p.chunk = max((int64_t)kMinTiles, (p.total + ranges - 1) / ranges);
+  p.chunk = max(kMinTiles, (int)(((unsigned)p.total + ranges - 1) / (unsigned)ranges));
   *in_front = front * p.jobs;
   return p;
 }
@@ -95,26 +94,26 @@ struct Cursor {
   SeqTiles s;
 };
 template <int TT>
-__device__ __forceinline__ Cursor find_tile(const ms_kv4_cache& c, const ms_kv4_attn& a, const Plan& p, int64_t u) {
+__device__ __forceinline__ Cursor find_tile(const ms_kv4_cache& c, const ms_kv4_attn& a, const Plan& p, int u) {
   const int lane = threadIdx.x & 31;
   Cursor k;
-  int64_t at = 0;
+  int at = 0;
   for (int b = 0; b < c.n_seqs; b += 32) {
-    const int64_t n = b + lane < c.n_seqs ? (int64_t)seq_tiles<TT>(c, a, b + lane).units() * p.jobs : 0;
-    int64_t inc = n;
+    const int n = b + lane < c.n_seqs ? seq_tiles<TT>(c, a, b + lane).units() * p.jobs : 0;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, u < at + inc);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      const int64_t in = u - at - __shfl_sync(0xffffffffu, inc - n, l);
+      const int in = u - at - __shfl_sync(0xffffffffu, inc - n, l);
       k.seq = b + l;
       k.s = seq_tiles<TT>(c, a, k.seq);
-      k.job = (int)(in / k.s.units());
-      k.tile = (int)(in - (int64_t)k.job * k.s.units());
+      k.job = in / k.s.units();
+      k.tile = in - k.job * k.s.units();
       return k;
     }
     at += __shfl_sync(0xffffffffu, inc, 31);
@@ -395,17 +394,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<HD, NT>& sm = *reinterpret_cast<Smem<HD, NT>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  pdl_launch_dependents();
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&sm.full[warp][s], 1);
     fence_mbar_init();
   }
   __syncwarp();
-  int64_t unused;
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  int unused;
   const Plan plan = make_plan<TT>(c, a, row_tiles, gridDim.x, 0, &unused);
-  const int64_t u0 = (int64_t)blockIdx.x * plan.chunk;
-  if (u0 >= plan.total) return;
-  const int count = (int)min(plan.chunk, plan.total - u0);   // tiles of the range
+  if (blockIdx.x >= (plan.total + plan.chunk - 1u) / plan.chunk) return;
+  const int u0 = blockIdx.x * plan.chunk, count = min(plan.chunk, plan.total - u0);   // the range
   const int rep = a.heads / c.kv_heads, rows = a.n_query * rep;
   const int shift = 31 - __clz(c.page_tokens);               // page_tokens is a power of two
   const int window = a.window > 0 ? a.window : 0x7fffffff;
@@ -549,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
       if (next < count) fetch_next(stage);
     }
 
-    // ---- join the warps: all on the largest maximum, warps 2 and 3 into 0 and 1, those through shared memory ----
+    // ---- join the warps: all on the largest maximum, the upper half of them into the lower half ----
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     // tile k of the product, rows g and g + 8: dims 2 k and 2 k + 1 of the lane's chunk
     auto place = [&](int r, int k) -> float2* {
       const int d = HD == 64 ? 8 * g + 2 * k : 128 * (k >> 3) + 16 * g + 2 * (k & 7);
-      return reinterpret_cast<float2*>(&sm.o[warp & 1][r][d]);
+      return reinterpret_cast<float2*>(&sm.o[warp % (kWarps / 2)][r][d]);
     };
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -601,8 +600,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     for (int i = threadIdx.x; i < ROWS * (HD / 4); i += kThreads) {
       const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, rr = row0 + r;
       if (rr >= rows) break;
-      const float4 x = *reinterpret_cast<const float4*>(&sm.o[0][r][d]), y = *reinterpret_cast<const float4*>(&sm.o[1][r][d]);
-      const float4 v = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      float4 v = *reinterpret_cast<const float4*>(&sm.o[0][r][d]);
+#pragma unroll
+      for (int w = 1; w < kWarps / 2; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+      }
       float top = sm.m[0][r], sum = 0.f;
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm.m[w][r]);
@@ -638,26 +641,26 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const ms_kv4_cache c
   __shared__ float ls[GROUPS], ms[GROUPS];
   const int jobs = c.kv_heads * row_tiles, seq = blockIdx.x / jobs, job = blockIdx.x % jobs, r = blockIdx.y;
   const int rep = a.heads / c.kv_heads, rr = (job % row_tiles) * ROWS + r;
-  int64_t base;
+  int base;
   const Plan plan = make_plan<TT>(c, a, row_tiles, ranges, seq, &base);
   const SeqTiles st = seq_tiles<TT>(c, a, seq);
-  const int64_t j0 = base + (int64_t)job * st.units(), j1 = j0 + st.n;
-  const int64_t c0 = j0 / plan.chunk, c1 = (j1 - 1) / plan.chunk;
+  const int j0 = base + job * st.units(), c0 = j0 / plan.chunk, c1 = (j0 + st.n - 1) / plan.chunk;
   pdl_wait_prior();                        // every block waits: this grid must not end before the first one
+  pdl_launch_dependents();
   if (c0 == c1 || rr >= a.n_query * rep) return;   // finished by its block, or no such row
   const int h = (job / row_tiles) * rep + rr % rep;
-  auto part = [&](int64_t b) { return (const float*)a.work + (b * 2 + (b == c0 ? 1 : 0)) * partial_floats<HD, ROWS>(); };
+  auto part = [&](int b) { return (const float*)a.work + ((int64_t)b * 2 + (b == c0 ? 1 : 0)) * partial_floats<HD, ROWS>(); };
   // a group of threads joins every GROUPS-th part on its own running maximum, kFlight loads under way at a time
   constexpr int kFlight = 8;
   const int col = threadIdx.x % COLS, grp = threadIdx.x / COLS;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = kNone, l = 0.f;
-  for (int64_t b0 = c0 + grp; b0 <= c1; b0 += GROUPS * kFlight) {
+  for (int b0 = c0 + grp; b0 <= c1; b0 += GROUPS * kFlight) {
     float4 x[kFlight];
     float pm[kFlight], pl[kFlight], top = m;
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      const int64_t b = b0 + i * GROUPS;
+      const int b = b0 + i * GROUPS;
       pm[i] = kNone;
       pl[i] = 0.f;
       x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -714,18 +717,21 @@ cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_attn& a, 
   const int smem = sizeof(Smem<HD, NT>);
   cudaError_t e = cudaFuncSetAttribute(kv4_attn_kernel<T, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kv4_attn_kernel<T, HD, NT><<<ranges_of(d, HD, NT), kThreads, smem, s>>>(c, a, row_tiles, d.err);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(c.n_seqs * c.kv_heads * row_tiles, min(rows, 8 * NT));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = s;
+  // both kernels start while their predecessor ends and wait for it on the device
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(ranges_of(d, HD, NT));
+  cfg.dynamicSmemBytes = smem;
+  e = cudaLaunchKernelEx(&cfg, kv4_attn_kernel<T, HD, NT>, c, a, row_tiles, d.err);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(c.n_seqs * c.kv_heads * row_tiles, min(rows, 8 * NT));
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, HD, NT>, c, a, row_tiles, ranges_of(d, HD, NT));
 }
 

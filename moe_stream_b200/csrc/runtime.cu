@@ -1763,6 +1763,10 @@ ms_status check_kv4_shape(const ms_kv4_cache& c, int n_query, int heads, const c
   if (n_query <= 0 || heads <= 0 || heads % c.kv_heads || (int64_t)n_query * (heads / c.kv_heads) > 128)
     return *why = "n_query > 0, heads a multiple of kv_heads, n_query * heads / kv_heads <= 128 required", MS_ERR_SHAPE;
   if ((int64_t)c.n_seqs * n_query * heads > 0x7fffff00ll / 32 || c.n_seqs > 65535) return *why = "too many rows", MS_ERR_SHAPE;
+  // tiles of 4096 / head_dim tokens, for each kv head and 8 rows (the split counts them in 32 bits)
+  const double tiles = (double)c.max_pages * c.page_tokens / (4096 / c.head_dim) + 16;
+  if (tiles * c.n_seqs * c.kv_heads * ((n_query * (heads / c.kv_heads) + 7) / 8) > 2.0e9)
+    return *why = "the capacity of all sequences is too large", MS_ERR_SHAPE;
   return MS_OK;
 }
 
