@@ -1,69 +1,435 @@
 // kernels_prompt_attn.cu — causal attention of packed sequences of different lengths (grouped heads, sliding
-// window, sinks, keys of a cached prefix in front of the queries).
+// window, sinks, keys of a cached prefix in front of the queries), on the 5th-generation tensor cores.
+//
+//   out = sum_j p_j v_j / (sum_j p_j + exp(sink - m)),  p_j = exp(scale q . k_j - m)
+//
+// A query tile is 128 rows: all heads of one kv head's group for 128 / group tokens, so that K and V are read
+// once for the group and short sequences still fill a tile.  A block holds NQ query tiles of one sequence (2; 1
+// with 256 dims, whose output takes half of the tensor memory) and walks over the keys in tiles of BN.
+//
+// Warps: NQ groups of 4 for the softmax, one that issues the MMAs, one that issues the TMA copies.  Steps
+// s = 0, 1, ... alternate between two score buffers in tensor memory: with NQ = 2 step s is query tile s & 1 and
+// key tile s / 2, with NQ = 1 it is key tile s.  The MMA warp issues scores(s + 2) right after values(s), so the
+// tensor core works on one buffer while the softmax works on the other.  A softmax thread owns a row: it reads
+// the scores, writes the probabilities over them as 16-bit pairs, and the value product takes them from tensor
+// memory.  The running maximum is raised only when a score exceeds it by more than 2^8, so that the output
+// is rarely rescaled; sums are in f32 over the unrounded probabilities.
+//
+// Values of keys behind the sequence's end (other rows of the packed buffer, perhaps not finite) are zeroed in
+// shared memory before the last product; their scores are masked.
+#include <cuda.h>
+
+#include <type_traits>
+
 #include "../../include/moestream_cuda.h"
 #include "attn_types.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "umma.cuh"
 
 namespace ms {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNone = -1e30f;   // the running maximum before any key
+constexpr float kRaise = 8.0f;    // log2 by which a score may exceed the running maximum
 
-// one warp per (query, head): lanes hold the dims, keys in order with a running maximum and sum
+template <int HD>
+struct Shape {
+  static constexpr int NQ = HD == 256 ? 1 : 2;          // query tiles of a block
+  static constexpr int BN = HD == 256 ? 64 : 128;       // keys of a tile
+  static constexpr int STAGES = HD == 64 ? 4 : 2;       // of K and of V
+  static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = BN * HD * 2;
+  static constexpr int SOFTMAX_WARPS = 4 * NQ, THREADS = 32 * (SOFTMAX_WARPS + (NQ == 2 ? 4 : 2));
+  static constexpr int SMEM = 1024 + NQ * Q_BYTES + 2 * STAGES * KV_BYTES;
+  static constexpr uint32_t O_COL = 2 * BN;             // columns of tensor memory: two score buffers, then the outputs
+  static constexpr uint32_t COLS = 512;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// where a block works
+struct Place {
+  int seq, q0, q1, k0, k1;   // rows of the sequence
+  int t0;                    // first token of the block
+  int tiles, first;          // key tiles, and the first one's index in the sequence
+  bool ok;
+};
+template <int HD>
+__device__ __forceinline__ Place find_place(const ms_prompt_attn& a, int n_tok, int index, uint32_t* err) {
+  using S = Shape<HD>;
+  const int lane = threadIdx.x & 31, per = S::NQ * n_tok;
+  Place p;
+  p.ok = false;
+  // blocks of all sequences; this one counts from the last, so that the longest rows of a prompt start first
+  int total = 0;
+  for (int b = 0; b < a.n_seqs; b += 32) {
+    const int i = b + lane;
+    const int n = i < a.n_seqs ? (max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) + per - 1) / per : 0;
+    total += __reduce_add_sync(0xffffffffu, n);
+  }
+  index = total - 1 - index;
+  if (index < 0) return p;
+  int at = 0;
+  for (int b = 0; b < a.n_seqs; b += 32) {
+    const int i = b + lane;
+    const int n = i < a.n_seqs ? (max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) + per - 1) / per : 0;
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, index < at + inc);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      p.seq = b + l;
+      p.t0 = (index - at - __shfl_sync(0xffffffffu, inc - n, l)) * per;
+      break;
+    }
+    at += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  p.q0 = a.cu_q[p.seq]; p.q1 = a.cu_q[p.seq + 1];
+  p.k0 = a.cu_k[p.seq]; p.k1 = a.cu_k[p.seq + 1];
+  if (p.q0 < 0 || p.q1 > a.total_q || p.k0 < 0 || p.k1 < p.k0 || p.k1 > a.total_k) {
+    if (threadIdx.x == 0) atomicOr(err, EF_BAD_INDEX);
+    return p;
+  }
+  const int nk = p.k1 - p.k0, nq = p.q1 - p.q0;
+  const int hi = nk - nq + min(nq, p.t0 + per) - 1;      // last key of the block's last query
+  const int lo = a.window > 0 ? max(0, nk - nq + p.t0 - a.window + 1) : 0;
+  p.first = lo / S::BN;
+  p.tiles = hi < lo ? 0 : hi / S::BN - p.first + 1;
+  p.ok = true;
+  return p;
+}
+
 template <class T, int HD>
-__global__ void __launch_bounds__(kWarps * 32) prompt_attn_kernel(const ms_prompt_attn a, uint32_t* err) {
-  constexpr int N = HD / 32;
-  const int lane = threadIdx.x & 31, h = blockIdx.y, g = h / (a.heads / a.kv_heads);
-  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (row >= a.total_q) return;
-  const int seq = seq_of_row(a.cu_q, a.n_seqs, row);
-  if (seq < 0) return;
-  const int k0 = a.cu_k[seq], k1 = a.cu_k[seq + 1];
-  if (k0 < 0 || k1 < k0 || k1 > a.total_k) {
-    if (lane == 0) atomicOr(err, EF_BAD_INDEX);
-    return;
+__global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
+    prompt_attn_kernel(const ms_prompt_attn a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map, int n_tok, uint32_t* err) {
+  using S = Shape<HD>;
+  constexpr int NQ = S::NQ, BN = S::BN, ST = S::STAGES, BLK = HD / 64;   // BLK: blocks of 64 dims
+  constexpr bool BF16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t *sq = sm, *sk = sq + NQ * S::Q_BYTES, *sv = sk + ST * S::KV_BYTES;
+  __shared__ uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[NQ];
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.x % a.kv_heads, rep = a.heads / a.kv_heads;
+  const Place pl = find_place<HD>(a, n_tok, blockIdx.x / a.kv_heads, err);
+  if (!pl.ok) return;
+
+  if (warp == S::SOFTMAX_WARPS) {
+    umma::tmem_alloc(&tmem_base, S::COLS);
+    umma::tmem_relinquish();
   }
-  const int last = k1 - (a.cu_q[seq + 1] - row), first = a.window > 0 ? max(k0, last - a.window + 1) : k0;
-  float qv[N], o[N], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) { qv[i] = to_f32(((const T*)a.q)[row * a.q_stride + h * HD + lane + 32 * i]); o[i] = 0.f; }
-  for (int j = first; j <= last; ++j) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(qv[i], to_f32(((const T*)a.k)[j * a.k_stride + g * HD + lane + 32 * i]), s);
-    s = warp_sum(s) * a.scale;
-    const float mn = fmaxf(m, s), f = expf(m - mn), p = expf(s - mn);
-    l = l * f + p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * f + p * to_f32(((const T*)a.v)[j * a.v_stride + g * HD + lane + 32 * i]);
-    m = mn;
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+    for (int i = 0; i < NQ; ++i) mbar_init(&o_full[i], 1);
+    fence_mbar_init();
   }
-  if (a.sinks) {
-    const float mn = fmaxf(m, a.sinks[h]), f = expf(m - mn);
-    l = l * f + expf(a.sinks[h] - mn);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const int nq = pl.q1 - pl.q0, nk = pl.k1 - pl.k0;
+  const int slots = NQ == 2 && pl.t0 + n_tok < nq ? 2 : 1;   // query tiles with rows
+  // steps: with NQ = 1 the two score buffers take the key tiles in turn
+  const int steps = NQ * pl.tiles;
+
+  // the two softmax groups need more than the 168 registers of 384 threads: 208 x 256 + 80 x 128 of 168 x 384
+  if (warp >= S::SOFTMAX_WARPS) {
+    if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == S::SOFTMAX_WARPS + 1) {
+      // ---- TMA ----
+      if (lane == 0 && pl.tiles > 0) {
+        const int rows = n_tok * rep;
+        mbar_expect_tx(&q_full, slots * BLK * rows * 128);
+        for (int i = 0; i < slots; ++i)
+          for (int b = 0; b < BLK; ++b)
+            tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + i * n_tok, &q_full);
+        bool alive = true;
+        for (int j = 0; j < pl.tiles && alive; ++j) {
+          const int st = j % ST, z = pl.k0 + (pl.first + j) * BN;
+          if (j >= ST) alive = mbar_wait(&k_empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY);
+          if (!alive) break;
+          mbar_expect_tx(&k_full[st], S::KV_BYTES);
+          for (int b = 0; b < BLK; ++b) tma_3d(sk + st * S::KV_BYTES + b * BN * 128, &k_map, 64 * b, head, z, &k_full[st]);
+          if (j >= ST) alive = mbar_wait(&v_empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY);
+          if (!alive) break;
+          mbar_expect_tx(&v_full[st], S::KV_BYTES);
+          for (int b = 0; b < BLK; ++b) tma_3d(sv + st * S::KV_BYTES + b * BN * 128, &v_map, 64 * b, head, z, &v_full[st]);
+        }
+        // nothing of this block may still be on its way when it ends (the copies of an unfinished walk, too)
+        if (!alive) {
+          mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
+          for (int i = 0; i < ST; ++i) { mbar_wait(&k_full[i], 0, nullptr, 0); mbar_wait(&v_full[i], 0, nullptr, 0); }
+        }
+      }
+    } else if (warp == S::SOFTMAX_WARPS) {
+      // ---- MMA: the whole warp walks, lane 0 issues ----
+      constexpr uint32_t id_s = umma::idesc_f16(128, BN, BF16, false), id_o = umma::idesc_f16(128, HD, BF16, true);
+      auto scores = [&](int s) {
+        const int slot = s & 1, j = NQ == 2 ? s >> 1 : s, st = j % ST;
+        if (lane == 0) {
+          const uint8_t* q = sq + (NQ == 2 ? slot : 0) * S::Q_BYTES;
+          const uint8_t* k = sk + st * S::KV_BYTES;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] *= f;
+          for (int b = 0; b < BLK; ++b)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma::mma_bf16(tmem + slot * BN, umma::smem_desc_sw128(q + b * 128 * 128 + kk * 32, 0),
+                             umma::smem_desc_sw128(k + b * BN * 128 + kk * 32, 0), id_s, b || kk);
+          umma::commit(&s_full[slot]);
+        }
+        __syncwarp();
+      };
+      auto free_stage = [&](uint64_t* bar, int j) {            // only where a copy waits for it: none is left open at the end
+        if (lane == 0 && j + ST < pl.tiles) umma::commit(bar);
+        __syncwarp();
+      };
+      // keys of tile j: waited for when its first scores are issued, released with its last
+      // (a wait that runs out does so for the whole warp)
+      auto wait = [&](uint64_t* bar, int parity) {
+        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
+      };
+      bool alive = pl.tiles > 0 && wait(&q_full, 0);
+      auto issue_scores = [&](int s) {
+        const int slot = s & 1, j = NQ == 2 ? s >> 1 : s, st = j % ST;
+        if (NQ == 1 || slot == 0) {
+          alive = wait(&k_full[st], j / ST);
+          umma::fence_after_sync();
+        }
+        if (!alive) return;
+        if (NQ == 1 || slot < slots) scores(s);
+        if (NQ == 1 || slot == 1) free_stage(&k_empty[st], j);
+      };
+      for (int s = 0; s < 2 && s < steps && alive; ++s) issue_scores(s);
+      for (int s = 0; s < steps && alive; ++s) {
+        const int slot = s & 1, j = NQ == 2 ? s >> 1 : s, st = j % ST;
+        const uint8_t* v = sv + st * S::KV_BYTES;
+        if (NQ == 1 || slot == 0) {
+          alive = wait(&v_full[st], j / ST);
+          if (!alive) break;
+          const int keys = nk - (pl.first + j) * BN;           // keys of the sequence in this tile
+          if (keys < BN) {                                     // the rest are rows of others: zeroed (16-byte units of 128-byte rows)
+            for (int i = lane; i < (BN - keys) * 8 * BLK; i += 32) {
+              const int b = i / ((BN - keys) * 8), u = i % ((BN - keys) * 8);
+              *reinterpret_cast<uint4*>(const_cast<uint8_t*>(v) + b * BN * 128 + keys * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+            }
+            umma::fence_proxy_async_smem();
+            __syncwarp();
+          }
+        }
+        if (NQ == 1 || slot < slots) {
+          const int turn = NQ == 2 ? j : s >> 1;               // how often this buffer was filled before
+          alive = wait(&p_full[slot], turn);
+          if (!alive) break;
+          umma::fence_after_sync();
+          if (lane == 0) {
+            const uint32_t o = tmem + S::O_COL + (NQ == 2 ? slot * HD : 0);
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk)
+              umma::mma_f16_ts(o, tmem + slot * BN + kk * 8, umma::smem_desc_sw128(v + kk * 2048, BN * 128), id_o, j > 0 || kk > 0);
+            umma::commit(&o_full[NQ == 2 ? slot : 0]);
+          }
+          __syncwarp();
+        }
+        if (NQ == 1 || slot == 1) free_stage(&v_empty[st], j);
+        if (s + 2 < steps) issue_scores(s + 2);
+      }
+    }
+  } else {
+    // ---- softmax: thread = row ----
+    if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int tile = warp >> 2, r = threadIdx.x & 127;       // query tile of the block, row of it
+    const int tok = pl.t0 + tile * n_tok + r / rep;          // token of the sequence
+    const bool row_ok = r < n_tok * rep && tok < nq;
+    const int h = head * rep + r % rep;
+    const int last = row_ok ? nk - nq + tok : -1;            // the row's last key
+    const int lo = a.window > 0 ? max(0, last - a.window + 1) : 0;
+    const float c2 = fmaxf(a.scale * kLog2e, 1e-37f);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t o_col = tmem + lanes + S::O_COL + (NQ == 2 ? tile * HD : 0);
+    float m = kNone, l = 0.f;
+    bool alive = true;
+    auto wait = [&](uint64_t* bar, int parity) {
+      return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
+    };
+    if (tile < slots) {
+      for (int j = 0; j < pl.tiles; ++j) {
+        const int slot = NQ == 2 ? tile : j & 1, turn = NQ == 2 ? j : j >> 1;
+        alive = wait(&s_full[slot], turn);
+        if (!alive) break;
+        umma::fence_after_sync();
+        const uint32_t s_col = tmem + lanes + slot * BN;
+        uint32_t u[BN];
+#pragma unroll
+        for (int i = 0; i < BN / 32; ++i) umma::ld_32x32b_x32_async(s_col + 32 * i, u + 32 * i);
+        umma::wait_ld();
+#pragma unroll
+        for (int i = 0; i < BN / 32; ++i) umma::loaded(u + 32 * i);
+        const int key0 = (pl.first + j) * BN;
+        if (!__all_sync(0xffffffffu, key0 >= lo && key0 + BN - 1 <= last)) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (key0 + i > last || key0 + i < lo) u[i] = 0xFF800000u;   // -inf
+        }
+        float top = __uint_as_float(u[0]);
+#pragma unroll
+        for (int i = 1; i < BN; ++i) top = fmaxf(top, __uint_as_float(u[i]));
+        top *= c2;
+        const bool raise = top > m + kRaise;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = raise ? top : m, f = exp2_fast(m - mn);
+          m = mn;
+          l *= f;
+          if (j > 0) {
+            // all value products of this output so far have to be done: with NQ = 2 the scores' arrival says so
+            if (NQ == 1) alive = wait(&o_full[0], j - 1);
+            if (!alive) break;
+            umma::fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+              uint32_t o[32];
+              umma::ld_32x32b_x32_async(o_col + 32 * i, o);
+              umma::wait_ld();
+              umma::loaded(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              umma::st_32x32b_x32(o_col + 32 * i, o);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < BN; i += 2) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(u[i]), c2, -m)), p1 = exp2_fast(fmaf(__uint_as_float(u[i + 1]), c2, -m));
+          l += p0 + p1;
+          u[i / 2] = pack2<T>(p0, p1);
+        }
+#pragma unroll
+        for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(s_col + 32 * i, u + 32 * i);
+        umma::wait_st();
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[slot]);
+      }
+      // ---- output ----
+      if (pl.tiles > 0 && alive) alive = wait(&o_full[NQ == 2 ? tile : 0], pl.tiles - 1);
+      umma::fence_after_sync();
+      float f = 0.f;
+      if (l > 0.f) {
+        float den = l;
+        f = 1.f;
+        if (a.sinks) {
+          const float sink = a.sinks[h < a.heads ? h : 0] * kLog2e, mm = fmaxf(m, sink);
+          f = exp2_fast(m - mm);
+          den = l * f + exp2_fast(sink - mm);
+        }
+        f /= den;
+      }
+      T* dst = (T*)a.out + (int64_t)(pl.q0 + tok) * a.out_stride + h * HD;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        uint32_t o[32];
+        if (pl.tiles > 0 && alive) {
+          umma::ld_32x32b_x32_async(o_col + 32 * i, o);
+          umma::wait_ld();
+          umma::loaded(o);
+        }
+        if (row_ok && alive) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = l > 0.f || l != l ? __uint_as_float(o[e + k]) * f : 0.f;
+            store8(dst + 32 * i + e, x);
+          }
+        }
+      }
+    }
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    ((T*)a.out)[row * a.out_stride + h * HD + lane + 32 * i] = from_f32<T>(l > 0.f ? o[i] / l : 0.f);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  if (warp == S::SOFTMAX_WARPS) umma::tmem_dealloc(tmem, S::COLS);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+
+// [tokens][heads][hd] with `stride` elements between tokens; boxes of 64 dims, `heads_box` heads, `tokens_box` tokens
+bool make_map(CUtensorMap* map, bool bf16, const void* p, int hd, int heads, int tokens, int64_t stride, int heads_box,
+              int tokens_box) {
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)tokens};
+  const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)heads_box, (cuuint32_t)tokens_box}, unit[3] = {1, 1, 1};
+  return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p), dims,
+                   strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int HD>
+cudaError_t start(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
+  using S = Shape<HD>;
+  const int rep = a.heads / a.kv_heads, n_tok = 128 / rep;
+  const bool bf16 = a.type == MS_Q_BF16;
+  if (!encoder()) return cudaErrorNotSupported;
+  CUtensorMap q, k, v;
+  if (!make_map(&q, bf16, a.q, HD, a.heads, a.total_q, a.q_stride, rep, n_tok)) return cudaErrorInvalidValue;
+  if (a.total_k == 0) k = v = q;   // no block has a key tile
+  else if (!make_map(&k, bf16, a.k, HD, a.kv_heads, a.total_k, a.k_stride, 1, S::BN) ||
+           !make_map(&v, bf16, a.v, HD, a.kv_heads, a.total_k, a.v_stride, 1, S::BN))
+    return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(prompt_attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e != cudaSuccess) return e;
+  // blocks of all sequences: at most one that is not full for each
+  const int64_t blocks = ((int64_t)a.total_q / (S::NQ * n_tok) + a.n_seqs) * a.kv_heads;
+  prompt_attn_kernel<T, HD><<<(unsigned)blocks, S::THREADS, S::SMEM, s>>>(a, q, k, v, n_tok, d.err);
+  return cudaGetLastError();
 }
 
 template <class T>
-cudaError_t start(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
-  const dim3 grid((a.total_q + kWarps - 1) / kWarps, a.heads);
-  if (a.head_dim == 64) prompt_attn_kernel<T, 64><<<grid, kWarps * 32, 0, s>>>(a, d.err);
-  else if (a.head_dim == 128) prompt_attn_kernel<T, 128><<<grid, kWarps * 32, 0, s>>>(a, d.err);
-  else prompt_attn_kernel<T, 256><<<grid, kWarps * 32, 0, s>>>(a, d.err);
-  return cudaGetLastError();
+cudaError_t start_hd(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
+  if (a.head_dim == 64) return start<T, 64>(d, a, s);
+  if (a.head_dim == 128) return start<T, 128>(d, a, s);
+  return start<T, 256>(d, a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_prompt_attention(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
   if (a.total_q == 0 || a.n_seqs == 0) return cudaSuccess;
-  return a.type == MS_Q_F16 ? start<__half>(d, a, s) : start<__nv_bfloat16>(d, a, s);
+  return a.type == MS_Q_F16 ? start_hd<__half>(d, a, s) : start_hd<__nv_bfloat16>(d, a, s);
 }
 
 }  // namespace ms
