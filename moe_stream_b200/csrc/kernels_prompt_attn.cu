@@ -42,8 +42,11 @@ struct Shape {
   static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = BN * HD * 2;
   static constexpr int SOFTMAX_WARPS = 4 * NQ, THREADS = 32 * (SOFTMAX_WARPS + (NQ == 2 ? 4 : 2));
   static constexpr int SMEM = 1024 + NQ * Q_BYTES + 2 * STAGES * KV_BYTES;
-  static constexpr uint32_t O_COL = 2 * BN;             // columns of tensor memory: two score buffers, then the outputs
+  // columns of tensor memory: two score buffers, the outputs, and (but for 128 dims, which fill all 512 columns)
+  // the probabilities of the two buffers; with 128 dims they take the first half of the scores they came from
+  static constexpr uint32_t O_COL = 2 * BN, P_COL = HD == 128 ? 0 : O_COL + NQ * HD, P_STEP = HD == 128 ? BN : BN / 2;
   static constexpr uint32_t COLS = 512;
+  static constexpr int POLY = 1, POLY_OF = 4;           // of so many pairs of exponentials, that many are polynomials
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -57,6 +60,60 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
           smem_u32(dst)),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+
+// ---- pairs of f32 in one 64-bit register (one instruction for both) ----
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(a));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x for a pair on the multiply-add pipe, which has time to spare while the special-function pipe computes the others:
+// x = n + f with n = round(x), f in [-1/2, 1/2], 2^f by a polynomial of least relative error (7.5e-5 with
+// degree 3, for bf16 probabilities; 2.7e-6 with degree 4, for f16), n added to the exponent.  x <= 9; below -126
+// the result is 2^-126 or so instead of 0.
+template <bool DEG4>
+__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
+  const float2 xc = unpair(x2);
+  const uint64_t x = pair(fmaxf(xc.x, -126.f), fmaxf(xc.y, -126.f));
+  const float magic = 12582912.f;                       // 1.5 * 2^23: adding it rounds to an integer in the low bits
+  const uint64_t y = add2(x, pair(magic, magic));
+  const uint64_t n = add2(y, pair(-magic, -magic));
+  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
+  uint64_t p;
+  if (DEG4) {
+    p = fma2(f, pair(0.009570100344717503f, 0.009570100344717503f), pair(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  } else {
+    p = fma2(f, pair(0.0551716573536396f, 0.0551716573536396f), pair(0.2426111251115799f, 0.2426111251115799f));
+    p = fma2(p, f, pair(0.6932609677314758f, 0.6932609677314758f));
+    p = fma2(p, f, pair(0.9999280571937561f, 0.9999280571937561f));
+  }
+  const float2 yf = unpair(y), pf = unpair(p);
+  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(yf.x) << 23)),
+                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(yf.y) << 23)));
 }
 
 // where a block works
@@ -149,11 +206,10 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  const uint32_t tmem = tmem_base;
+  constexpr uint32_t tmem = 0;             // all 512 columns are this block's, so they start at 0
+  if (threadIdx.x == 0 && tmem_base != tmem) atomicOr(err, EF_BAD_SHAPE);
   const int nq = pl.q1 - pl.q0, nk = pl.k1 - pl.k0;
   const int slots = NQ == 2 && pl.t0 + n_tok < nq ? 2 : 1;   // query tiles with rows
-  // steps: with NQ = 1 the two score buffers take the key tiles in turn
-  const int steps = NQ * pl.tiles;
 
   // the two softmax groups need more than the 168 registers of 384 threads: 208 x 256 + 80 x 128 of 168 x 384
   if (warp >= S::SOFTMAX_WARPS) {
@@ -187,74 +243,84 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
     } else if (warp == S::SOFTMAX_WARPS) {
       // ---- MMA: the whole warp walks, lane 0 issues ----
       constexpr uint32_t id_s = umma::idesc_f16(128, BN, BF16, false), id_o = umma::idesc_f16(128, HD, BF16, true);
-      auto scores = [&](int s) {
-        const int slot = s & 1, j = NQ == 2 ? s >> 1 : s, st = j % ST;
-        if (lane == 0) {
-          const uint8_t* q = sq + (NQ == 2 ? slot : 0) * S::Q_BYTES;
-          const uint8_t* k = sk + st * S::KV_BYTES;
-#pragma unroll
-          for (int b = 0; b < BLK; ++b)
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma::mma_bf16(tmem + slot * BN, umma::smem_desc_sw128(q + b * 128 * 128 + kk * 32, 0),
-                             umma::smem_desc_sw128(k + b * BN * 128 + kk * 32, 0), id_s, b || kk);
-          umma::commit(&s_full[slot]);
-        }
+      // descriptors of the first tiles; others are that many 16-byte units further
+      const uint64_t dq = umma::smem_desc_sw128(sq, 0), dk = umma::smem_desc_sw128(sk, 0), dv = umma::smem_desc_sw128(sv, BN * 128);
+      const bool one = umma::elect();
+      auto free_stage = [&](uint64_t* bar, int j) {          // only where a copy waits for it: none is left open at the end
+        if (one && j + ST < pl.tiles) umma::commit(bar);
         __syncwarp();
       };
-      auto free_stage = [&](uint64_t* bar, int j) {            // only where a copy waits for it: none is left open at the end
-        if (lane == 0 && j + ST < pl.tiles) umma::commit(bar);
-        __syncwarp();
-      };
-      // keys of tile j: waited for when its first scores are issued, released with its last
       // (a wait that runs out does so for the whole warp)
       auto wait = [&](uint64_t* bar, int parity) {
         return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
       };
       bool alive = pl.tiles > 0 && wait(&q_full, 0);
-      auto issue_scores = [&](int s) {
-        const int slot = s & 1, j = NQ == 2 ? s >> 1 : s, st = j % ST;
+      // slot is a constant: its addresses are, too (a block issues an MMA every 64 cycles)
+      auto scores = [&](auto slot_c, int j) {
+        constexpr int slot = decltype(slot_c)::value;
+        if (!alive || j >= pl.tiles) return;
+        const int st = j % ST;
         if (NQ == 1 || slot == 0) {
           alive = wait(&k_full[st], j / ST);
+          if (!alive) return;
           umma::fence_after_sync();
         }
-        if (!alive) return;
-        if (NQ == 1 || slot < slots) scores(s);
+        if (NQ == 1 || slot < slots) {
+          if (one) {
+            const uint64_t q = dq + (NQ == 2 ? slot : 0) * (S::Q_BYTES >> 4), k = dk + st * (S::KV_BYTES >> 4);
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                umma::mma_bf16(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, k + (b * BN * 128 + kk * 32) / 16, id_s, b || kk);
+            umma::commit(&s_full[slot]);
+          }
+          __syncwarp();
+        }
         if (NQ == 1 || slot == 1) free_stage(&k_empty[st], j);
       };
-      for (int s = 0; s < 2 && s < steps && alive; ++s) issue_scores(s);
-      for (int s = 0; s < steps && alive; ++s) {
-        const int slot = s & 1, j = NQ == 2 ? s >> 1 : s, st = j % ST;
-        const uint8_t* v = sv + st * S::KV_BYTES;
+      auto values = [&](auto slot_c, int j) {
+        constexpr int slot = decltype(slot_c)::value;
+        if (!alive || j >= pl.tiles) return;
+        const int st = j % ST;
         if (NQ == 1 || slot == 0) {
           alive = wait(&v_full[st], j / ST);
-          if (!alive) break;
+          if (!alive) return;
           const int keys = nk - (pl.first + j) * BN;           // keys of the sequence in this tile
           if (keys < BN) {                                     // the rest are rows of others: zeroed (16-byte units of 128-byte rows)
             for (int i = lane; i < (BN - keys) * 8 * BLK; i += 32) {
               const int b = i / ((BN - keys) * 8), u = i % ((BN - keys) * 8);
-              *reinterpret_cast<uint4*>(const_cast<uint8_t*>(v) + b * BN * 128 + keys * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(sv + st * S::KV_BYTES + b * BN * 128 + keys * 128 + u * 16) = make_uint4(0, 0, 0, 0);
             }
             umma::fence_proxy_async_smem();
             __syncwarp();
           }
         }
         if (NQ == 1 || slot < slots) {
-          const int turn = NQ == 2 ? j : s >> 1;               // how often this buffer was filled before
-          alive = wait(&p_full[slot], turn);
-          if (!alive) break;
+          alive = wait(&p_full[slot], NQ == 2 ? j : j >> 1);   // how often this buffer was filled before
+          if (!alive) return;
           umma::fence_after_sync();
-          if (lane == 0) {
-            const uint32_t o = tmem + S::O_COL + (NQ == 2 ? slot * HD : 0);
+          if (one) {
+            const uint64_t v = dv + st * (S::KV_BYTES >> 4);
 #pragma unroll
             for (int kk = 0; kk < BN / 16; ++kk)
-              umma::mma_f16_ts(o, tmem + slot * BN + kk * 8, umma::smem_desc_sw128(v + kk * 2048, BN * 128), id_o, j > 0 || kk > 0);
+              umma::mma_f16_ts(S::O_COL + (NQ == 2 ? slot * HD : 0), S::P_COL + slot * S::P_STEP + kk * 8, v + kk * 2048 / 16, id_o, j > 0 || kk > 0);
             umma::commit(&o_full[NQ == 2 ? slot : 0]);
           }
           __syncwarp();
         }
         if (NQ == 1 || slot == 1) free_stage(&v_empty[st], j);
-        if (s + 2 < steps) issue_scores(s + 2);
+      };
+      constexpr std::integral_constant<int, 0> s0;
+      constexpr std::integral_constant<int, 1> s1;
+      scores(s0, 0);
+      scores(s1, NQ == 2 ? 0 : 1);
+      for (int j = 0; j < pl.tiles && alive; j += NQ == 2 ? 1 : 2) {
+        const int j1 = NQ == 2 ? j : j + 1, ahead = NQ == 2 ? 1 : 2;
+        values(s0, j);
+        scores(s0, j + ahead);
+        values(s1, j1);
+        scores(s1, j1 + ahead);
       }
     }
   } else {
@@ -280,7 +346,7 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
         alive = wait(&s_full[slot], turn);
         if (!alive) break;
         umma::fence_after_sync();
-        const uint32_t s_col = tmem + lanes + slot * BN;
+        const uint32_t s_col = tmem + lanes + slot * BN, p_col = tmem + lanes + S::P_COL + slot * S::P_STEP;
         uint32_t u[BN];
 #pragma unroll
         for (int i = 0; i < BN / 32; ++i) umma::ld_32x32b_x32_async(s_col + 32 * i, u + 32 * i);
@@ -293,10 +359,14 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
           for (int i = 0; i < BN; ++i)
             if (key0 + i > last || key0 + i < lo) u[i] = 0xFF800000u;   // -inf
         }
-        float top = __uint_as_float(u[0]);
+        float top4[4];                                       // four chains
 #pragma unroll
-        for (int i = 1; i < BN; ++i) top = fmaxf(top, __uint_as_float(u[i]));
-        top *= c2;
+        for (int i = 0; i < 4; ++i) top4[i] = fmaxf(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+#pragma unroll
+        for (int i = 8; i < BN; i += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], __uint_as_float(u[i + 2 * e]), __uint_as_float(u[i + 2 * e + 1]));
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c2;
         const bool raise = top > m + kRaise;
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = raise ? top : m, f = exp2_fast(m - mn);
@@ -319,20 +389,34 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
             }
           }
         }
+        const uint64_t c22 = pair(c2, c2), m22 = pair(-m, -m);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < BN; i += 2) {
-          const float p0 = exp2_fast(fmaf(__uint_as_float(u[i]), c2, -m)), p1 = exp2_fast(fmaf(__uint_as_float(u[i + 1]), c2, -m));
-          l += p0 + p1;
-          u[i / 2] = pack2<T>(p0, p1);
+          const uint64_t x = fma2(pair(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), c22, m22);
+          float2 e;
+          if (i / 2 % S::POLY_OF < S::POLY) {
+            e = exp2_poly<!BF16>(x);
+          } else {
+            e = unpair(x);
+            e.x = exp2_fast(e.x);
+            e.y = exp2_fast(e.y);
+          }
+          sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(e.x, e.y));
+          u[i / 2] = pack2<T>(e.x, e.y);
+          if (i % 64 == 62) umma::st_32x32b_x32(p_col + (i / 64) * 32, u + (i / 64) * 32);
         }
-#pragma unroll
-        for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(s_col + 32 * i, u + 32 * i);
+        const float2 both = unpair(add2(sum[0], sum[1]));
+        l += both.x + both.y;
         umma::wait_st();
         umma::fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[slot]);
       }
       // ---- output ----
+      // A wait on a phase's parity tells it from the one before only: the scores of tile j vouch for the value products
+      // up to j - 1 (NQ = 2) or j - 2, so with NQ = 1 the last but one is waited for first.
+      if (NQ == 1 && pl.tiles > 1 && alive) alive = wait(&o_full[0], pl.tiles - 2);
       if (pl.tiles > 0 && alive) alive = wait(&o_full[NQ == 2 ? tile : 0], pl.tiles - 1);
       umma::fence_after_sync();
       float f = 0.f;

@@ -420,6 +420,22 @@ def test_prompt_attention(ctx, case):
     assert torch.equal(out[:n], again[:n])
 
 
+@pytest.mark.parametrize("hd,H,kv,n,cached", [(64, 16, 2, 700, 900), (128, 8, 8, 900, 1300), (256, 16, 2, 700, 900)])
+def test_prompt_attention_gives_the_same_bits_every_time(ctx, hd, H, kv, n, cached):
+    """Many key tiles, sharp scores (the running maximum rises often): every product and rescaling is waited for."""
+    q, k, v, cq, ck, both, _ = prompt_case([n], [cached], H, kv, hd, torch.bfloat16, seed=6, behind=0)
+    q = q * 2
+    first = torch.empty_like(q)
+    ctx.prompt_attention(q, k, v, cq, ck, first)
+    ctx.sync()
+    want, tol = prompt_reference(q, k, v, [n], both, 0, hd ** -0.5, None)
+    within(first, want, tol)
+    for _ in range(40):
+        out = torch.empty_like(q)
+        ctx.prompt_attention(q, k, v, cq, ck, out)
+        assert torch.equal(out, first)
+
+
 def test_prompt_attention_neighbours_hold_nan_and_infinity(ctx):
     """What another sequence holds does not reach a sequence's rows."""
     new, H, kv, hd = [70, 90, 50], 8, 2, 128
