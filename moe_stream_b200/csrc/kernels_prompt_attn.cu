@@ -12,8 +12,9 @@
 // key tile s / 2, with NQ = 1 it is key tile s.  The MMA warp issues scores(s + 2) right after values(s), so the
 // tensor core works on one buffer while the softmax works on the other.  A softmax thread owns a row: it reads
 // the scores, writes the probabilities over them as 16-bit pairs, and the value product takes them from tensor
-// memory.  The running maximum is raised only when a score exceeds it by more than 2^8, so that the output
-// is rarely rescaled; sums are in f32 over the unrounded probabilities.
+// memory.  The running maximum is that of the row's first tile until the probabilities of a later one add up to more
+// than kRaise: only then the tile's maximum is looked for and the output rescaled, and no probability comes
+// near the largest f16.  Sums are in f32 over the unrounded probabilities.
 //
 // Values of keys behind the sequence's end (other rows of the packed buffer, perhaps not finite) are zeroed in
 // shared memory before the last product; their scores are masked.
@@ -32,7 +33,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;   // the running maximum before any key
-constexpr float kRaise = 8.0f;    // log2 by which a score may exceed the running maximum
+constexpr float kRaise = 4096.f;  // sum of a row's probabilities of a tile that raises the running maximum
 
 template <int HD>
 struct Shape {
@@ -46,7 +47,6 @@ struct Shape {
   // the probabilities of the two buffers; with 128 dims they take the first half of the scores they came from
   static constexpr uint32_t O_COL = 2 * BN, P_COL = HD == 128 ? 0 : O_COL + NQ * HD, P_STEP = HD == 128 ? BN : BN / 2;
   static constexpr uint32_t COLS = 512;
-  static constexpr int POLY = 1, POLY_OF = 4;           // of so many pairs of exponentials, that many are polynomials
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -88,34 +88,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x for a pair on the multiply-add pipe, which has time to spare while the special-function pipe computes the others:
-// x = n + f with n = round(x), f in [-1/2, 1/2], 2^f by a polynomial of least relative error (7.5e-5 with
-// degree 3, for bf16 probabilities; 2.7e-6 with degree 4, for f16), n added to the exponent.  x <= 9; below -126
-// the result is 2^-126 or so instead of 0.
-template <bool DEG4>
-__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
-  const float2 xc = unpair(x2);
-  const uint64_t x = pair(fmaxf(xc.x, -126.f), fmaxf(xc.y, -126.f));
-  const float magic = 12582912.f;                       // 1.5 * 2^23: adding it rounds to an integer in the low bits
-  const uint64_t y = add2(x, pair(magic, magic));
-  const uint64_t n = add2(y, pair(-magic, -magic));
-  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
-  uint64_t p;
-  if (DEG4) {
-    p = fma2(f, pair(0.009570100344717503f, 0.009570100344717503f), pair(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
-  } else {
-    p = fma2(f, pair(0.0551716573536396f, 0.0551716573536396f), pair(0.2426111251115799f, 0.2426111251115799f));
-    p = fma2(p, f, pair(0.6932609677314758f, 0.6932609677314758f));
-    p = fma2(p, f, pair(0.9999280571937561f, 0.9999280571937561f));
-  }
-  const float2 yf = unpair(y), pf = unpair(p);
-  return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(yf.x) << 23)),
-                     __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(yf.y) << 23)));
-}
-
 // where a block works
 struct Place {
   int seq, q0, q1, k0, k1;   // rows of the sequence
@@ -347,31 +319,54 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
         if (!alive) break;
         umma::fence_after_sync();
         const uint32_t s_col = tmem + lanes + slot * BN, p_col = tmem + lanes + S::P_COL + slot * S::P_STEP;
-        uint32_t u[BN];
-#pragma unroll
-        for (int i = 0; i < BN / 32; ++i) umma::ld_32x32b_x32_async(s_col + 32 * i, u + 32 * i);
-        umma::wait_ld();
-#pragma unroll
-        for (int i = 0; i < BN / 32; ++i) umma::loaded(u + 32 * i);
         const int key0 = (pl.first + j) * BN;
-        if (!__all_sync(0xffffffffu, key0 >= lo && key0 + BN - 1 <= last)) {
+        uint32_t u[BN];
+        auto load = [&]() {                                  // the scores, masked
 #pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (key0 + i > last || key0 + i < lo) u[i] = 0xFF800000u;   // -inf
-        }
-        float top4[4];                                       // four chains
+          for (int i = 0; i < BN / 32; ++i) umma::ld_32x32b_x32_async(s_col + 32 * i, u + 32 * i);
+          umma::wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top4[i] = fmaxf(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+          for (int i = 0; i < BN / 32; ++i) umma::loaded(u + 32 * i);
+          if (!__all_sync(0xffffffffu, key0 >= lo && key0 + BN - 1 <= last)) {
 #pragma unroll
-        for (int i = 8; i < BN; i += 8)
+            for (int i = 0; i < BN; ++i)
+              if (key0 + i > last || key0 + i < lo) u[i] = 0xFF800000u;   // -inf
+          }
+        };
+        auto raise_max = [&]() {                             // to the tile's, with the sum and the output so far
+          float top4[4];                                     // four chains
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], __uint_as_float(u[i + 2 * e]), __uint_as_float(u[i + 2 * e + 1]));
-        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c2;
-        const bool raise = top > m + kRaise;
-        if (__any_sync(0xffffffffu, raise)) {
-          const float mn = raise ? top : m, f = exp2_fast(m - mn);
-          m = mn;
+          for (int i = 0; i < 4; ++i) top4[i] = fmaxf(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+#pragma unroll
+          for (int i = 8; i < BN; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], __uint_as_float(u[i + 2 * e]), __uint_as_float(u[i + 2 * e + 1]));
+          const float top = fmaxf(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c2, m), f = exp2_fast(m - top);
+          m = top;
           l *= f;
+          return f;
+        };
+        auto exps = [&]() {                                  // u becomes pairs of probabilities; their sum
+          const uint64_t c22 = pair(c2, c2), m22 = pair(-m, -m);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int i = 0; i < BN; i += 2) {
+            float2 e = unpair(fma2(pair(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), c22, m22));
+            e.x = exp2_fast(e.x);
+            e.y = exp2_fast(e.y);
+            sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(e.x, e.y));
+            u[i / 2] = pack2<T>(e.x, e.y);
+          }
+          const float2 both = unpair(add2(sum[0], sum[1]));
+          return both.x + both.y;
+        };
+        load();
+        if (j == 0) raise_max();
+        float sum = exps();
+        if (__any_sync(0xffffffffu, sum > kRaise)) {         // (not with the first tile, whose maximum was taken)
+          load();
+          const float f = raise_max();
+          sum = exps();
           if (j > 0) {
             // all value products of this output so far have to be done: with NQ = 2 the scores' arrival says so
             if (NQ == 1) alive = wait(&o_full[0], j - 1);
@@ -389,25 +384,9 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
             }
           }
         }
-        const uint64_t c22 = pair(c2, c2), m22 = pair(-m, -m);
-        uint64_t sum[2] = {0, 0};
+        l += sum;
 #pragma unroll
-        for (int i = 0; i < BN; i += 2) {
-          const uint64_t x = fma2(pair(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), c22, m22);
-          float2 e;
-          if (i / 2 % S::POLY_OF < S::POLY) {
-            e = exp2_poly<!BF16>(x);
-          } else {
-            e = unpair(x);
-            e.x = exp2_fast(e.x);
-            e.y = exp2_fast(e.y);
-          }
-          sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(e.x, e.y));
-          u[i / 2] = pack2<T>(e.x, e.y);
-          if (i % 64 == 62) umma::st_32x32b_x32(p_col + (i / 64) * 32, u + (i / 64) * 32);
-        }
-        const float2 both = unpair(add2(sum[0], sum[1]));
-        l += both.x + both.y;
+        for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(p_col + 32 * i, u + 32 * i);
         umma::wait_st();
         umma::fence_before_sync();
         __syncwarp();
