@@ -39,13 +39,17 @@ template <int HD>
 struct Shape {
   static constexpr int NQ = HD == 256 ? 1 : 2;          // query tiles of a block
   static constexpr int BN = HD == 256 ? 64 : 128;       // keys of a tile
-  static constexpr int STAGES = HD == 64 ? 4 : 2;       // of K and of V
+  static constexpr int STAGES = HD == 64 ? 4 : HD == 128 ? 2 : 3;   // of K and of V
   static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = BN * HD * 2;
   static constexpr int SOFTMAX_WARPS = 4 * NQ, THREADS = 32 * (SOFTMAX_WARPS + (NQ == 2 ? 4 : 2));
-  static constexpr int SMEM = 1024 + NQ * Q_BYTES + 2 * STAGES * KV_BYTES;
-  // columns of tensor memory: two score buffers, the outputs, and (but for 128 dims, which fill all 512 columns)
-  // the probabilities of the two buffers; with 128 dims they take the first half of the scores they came from
-  static constexpr uint32_t O_COL = 2 * BN, P_COL = HD == 128 ? 0 : O_COL + NQ * HD, P_STEP = HD == 128 ? BN : BN / 2;
+  // NQ = 1: queries in tensor memory and probabilities in shared memory, so that the score product, whose tiles are
+  // half as wide, reads one operand from shared memory only (both would need 192 bytes a cycle of its 128)
+  static constexpr int P_BYTES = NQ == 1 ? 128 * BN * 2 : 0;
+  static constexpr int SMEM = 1024 + (NQ == 2 ? NQ * Q_BYTES : 2 * P_BYTES) + 2 * STAGES * KV_BYTES;
+  // columns of tensor memory: two score buffers, the outputs; then with 64 dims the probabilities of the two buffers
+  // (with 128 dims, which fill all 512 columns, they take the first half of the scores they came from), with 256
+  // dims the queries
+  static constexpr uint32_t O_COL = 2 * BN, P_COL = HD == 128 ? 0 : O_COL + NQ * HD, P_STEP = HD == 128 ? BN : BN / 2, Q_COL = O_COL + HD;
   static constexpr uint32_t COLS = 512;
 };
 
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
   constexpr bool BF16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *sq = sm, *sk = sq + NQ * S::Q_BYTES, *sv = sk + ST * S::KV_BYTES;
+  uint8_t *sq = sm, *sk = sq + (NQ == 2 ? NQ * S::Q_BYTES : 2 * S::P_BYTES), *sv = sk + ST * S::KV_BYTES;   // NQ = 1: sq holds probabilities
   __shared__ uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[NQ];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
     umma::tmem_relinquish();
   }
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1);
+    mbar_init(&q_full, NQ == 2 ? 1 : 4);
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
@@ -190,10 +194,12 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
       // ---- TMA ----
       if (lane == 0 && pl.tiles > 0) {
         const int rows = n_tok * rep;
-        mbar_expect_tx(&q_full, slots * BLK * rows * 128);
-        for (int i = 0; i < slots; ++i)
-          for (int b = 0; b < BLK; ++b)
-            tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + i * n_tok, &q_full);
+        if (NQ == 2) {
+          mbar_expect_tx(&q_full, slots * BLK * rows * 128);
+          for (int i = 0; i < slots; ++i)
+            for (int b = 0; b < BLK; ++b)
+              tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + i * n_tok, &q_full);
+        }
         bool alive = true;
         for (int j = 0; j < pl.tiles && alive; ++j) {
           const int st = j % ST, z = pl.k0 + (pl.first + j) * BN;
@@ -208,7 +214,7 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
         }
         // nothing of this block may still be on its way when it ends (the copies of an unfinished walk, too)
         if (!alive) {
-          mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
+          if (NQ == 2) mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
           for (int i = 0; i < ST; ++i) { mbar_wait(&k_full[i], 0, nullptr, 0); mbar_wait(&v_full[i], 0, nullptr, 0); }
         }
       }
@@ -243,8 +249,11 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
 #pragma unroll
             for (int b = 0; b < BLK; ++b)
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                umma::mma_bf16(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, k + (b * BN * 128 + kk * 32) / 16, id_s, b || kk);
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint64_t kd = k + (b * BN * 128 + kk * 32) / 16;
+                if (NQ == 2) umma::mma_bf16(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, kd, id_s, b || kk);
+                else umma::mma_f16_ts(slot * BN, S::Q_COL + (b * 4 + kk) * 8, kd, id_s, b || kk);
+              }
             umma::commit(&s_full[slot]);
           }
           __syncwarp();
@@ -275,8 +284,11 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
           if (one) {
             const uint64_t v = dv + st * (S::KV_BYTES >> 4);
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              umma::mma_f16_ts(S::O_COL + (NQ == 2 ? slot * HD : 0), S::P_COL + slot * S::P_STEP + kk * 8, v + kk * 2048 / 16, id_o, j > 0 || kk > 0);
+            for (int kk = 0; kk < BN / 16; ++kk) {
+              const uint64_t vd = v + kk * 2048 / 16;
+              if (NQ == 2) umma::mma_f16_ts(S::O_COL + slot * HD, S::P_COL + slot * S::P_STEP + kk * 8, vd, id_o, j > 0 || kk > 0);
+              else umma::mma_bf16(S::O_COL, dq + slot * (S::P_BYTES >> 4) + kk * 32 / 16, vd, id_o, j > 0 || kk > 0);
+            }
             umma::commit(&o_full[NQ == 2 ? slot : 0]);
           }
           __syncwarp();
@@ -312,6 +324,23 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
     auto wait = [&](uint64_t* bar, int parity) {
       return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
     };
+    if (NQ == 1 && pl.tiles > 0) {       // the row's queries to tensor memory, as they are
+      const uint4* src = reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(pl.q0 + tok) * a.q_stride + h * HD);
+#pragma unroll
+      for (int i = 0; i < HD / 64; ++i) {
+        uint32_t x[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 w = row_ok ? src[8 * i + e] : make_uint4(0, 0, 0, 0);
+          x[4 * e] = w.x; x[4 * e + 1] = w.y; x[4 * e + 2] = w.z; x[4 * e + 3] = w.w;
+        }
+        umma::st_32x32b_x32(tmem + lanes + S::Q_COL + 32 * i, x);
+      }
+      umma::wait_st();
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    }
     if (tile < slots) {
       for (int j = 0; j < pl.tiles; ++j) {
         const int slot = NQ == 2 ? tile : j & 1, turn = NQ == 2 ? j : j >> 1;
@@ -385,8 +414,16 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
           }
         }
         l += sum;
+        if (NQ == 2) {
 #pragma unroll
-        for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(p_col + 32 * i, u + 32 * i);
+          for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(p_col + 32 * i, u + 32 * i);
+        } else {                                             // a row of 64 keys is 128 bytes, 16-byte units permuted as TMA would
+          uint8_t* dst = sq + slot * S::P_BYTES + r * 128;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7)) << 4)) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+          umma::fence_proxy_async_smem();
+        }
         umma::wait_st();
         umma::fence_before_sync();
         __syncwarp();
