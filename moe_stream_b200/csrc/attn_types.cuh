@@ -45,6 +45,7 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
 template <class T>
 struct Raw8 {
   uint4 u;
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -59,6 +60,7 @@ struct Raw8 {
 template <>
 struct Raw8<float> {
   float4 a, b;
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void load(const float* p) {
     a = reinterpret_cast<const float4*>(p)[0];
     b = reinterpret_cast<const float4*>(p)[1];

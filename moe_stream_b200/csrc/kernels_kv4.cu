@@ -4,6 +4,8 @@
 // o + d (16 + c).  The hidden 16 makes a code the top mantissa bits of the f16 or bf16 number 16 + c, so the
 // attention kernel builds tensor-core operands from it with one mask-and-or.  The layout of a block of 16 tokens
 // is in include/moestream_cuda.h.  Both kernels are bound by memory: every row and every block byte moves once.
+#include <type_traits>
+
 #include "../../include/moestream_cuda.h"
 #include "attn_types.cuh"
 #include "common.cuh"
@@ -13,174 +15,268 @@
 namespace ms {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128, kRows = 16;   // rows of a block at most
 
-// 8 dims of a group of 32 held by 4 neighbouring lanes -> codes and the group's scales
-struct Group8 {
-  float d, o;
-  uint32_t c[8];
+// ---- which rows of the block lead a token pair of the cache (an even token, or the first row of a sequence), and where
+// their pair stands.  A pair's V codes share words, so the lanes that hold both tokens store whole words.  One
+// thread looks up a row for all heads. ----
+struct Leads {
+  int64_t block[kRows];   // the 16-token block of head 0, counted in blocks from the start of the pages
+  int row[kRows];
+  int tok[kRows];         // token in the block; + 16: the next row is the pair's other token
+  int n;
 };
-__device__ __forceinline__ Group8 quantise8(float (&x)[8]) {
+__device__ __forceinline__ void find_leads(const ms_kv4_cache& c, const ms_kv4_rows& r, int rows, Leads& ls, uint32_t* err) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, j = blockIdx.x * rows + lane;
+    bool lead = false;
+    int64_t block = 0;
+    int tok = 0;
+    if (lane < rows && j < r.total) {
+      const int i = seq_of_row(r.cu, c.n_seqs, j);
+      if (i >= 0) {
+        const int begin = r.cu[i], end = r.cu[i + 1], at = j - begin, pos = r.start[i] + at;
+        if (!(pos & 1) || at == 0) {
+          block = kv4_block(c, i, pos, 0);
+          lead = block >= 0;
+          if (!lead) atomicOr(err, EF_BAD_INDEX);
+          tok = (pos & 15) | (!(pos & 1) && j + 1 < end && j + 1 < r.total ? 16 : 0);
+        }
+      }
+    }
+    const unsigned mask = __ballot_sync(0xffffffffu, lead);
+    if (lead) {
+      const int k = __popc(mask & ((1u << lane) - 1));
+      ls.block[k] = block;
+      ls.row[k] = j;
+      ls.tok[k] = tok;
+    }
+    if (lane == 0) ls.n = __popc(mask);
+  }
+  __syncthreads();
+}
+
+// ---- quantising: 8 dims of a group of 32 held by 4 neighbouring lanes ----
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// whether a value is beyond +-16384, infinite or NaN
+template <class T>
+__device__ __forceinline__ bool unusual(const Raw8<T>& r) {
+  const uint32_t m = max_u16x2(max_u16x2(r.u.x & 0x7FFF7FFFu, r.u.y & 0x7FFF7FFFu), max_u16x2(r.u.z & 0x7FFF7FFFu, r.u.w & 0x7FFF7FFFu));
+  const uint32_t most = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7400u : 0x4680u;   // 16384 in f16 / bf16
+  return (m & 0xFFFFu) > most || (m >> 16) > most;
+}
+template <>
+__device__ __forceinline__ bool unusual<float>(const Raw8<float>& r) {
+  return !(fabsf(r.a.x) <= 16384.f && fabsf(r.a.y) <= 16384.f && fabsf(r.a.z) <= 16384.f && fabsf(r.a.w) <= 16384.f &&
+           fabsf(r.b.x) <= 16384.f && fabsf(r.b.y) <= 16384.f && fabsf(r.b.z) <= 16384.f && fabsf(r.b.w) <= 16384.f);
+}
+struct Group8 {
+  uint32_t scale;   // f16 d, f16 o
+  uint32_t c[8];    // 0x4B400000 + code
+};
+constexpr float kMagic = 12582912.f;   // 1.5 * 2^23, bits 0x4B400000: adding it rounds to an integer in the low bits
+template <class T>
+__device__ __forceinline__ Group8 quantise8(const Raw8<T>& raw) {
   Group8 g;
+  float x[8];
+  raw.get(x);
+  if (unusual(raw)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -16384.f), 16384.f);
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) { lo = fminf(lo, x[i]); hi = fmaxf(hi, x[i]); }
+    for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -16384.f), 16384.f);
+  }
+  float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+  float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
 #pragma unroll
   for (int m = 1; m <= 2; m <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
   }
   // d and o are rounded to f16 first and the codes computed from the rounded values
-  g.d = __half2float(__float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)));
-  g.o = __half2float(__float2half_rn(__fsub_rn(lo, 16.0f * g.d)));
+  const __half dh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+  const float d = __half2float(dh);
+  const __half oh = __float2half_rn(__fsub_rn(lo, 16.0f * d));
+  const float o = __half2float(oh);
+  g.scale = __half_as_ushort(dh) | (uint32_t)__half_as_ushort(oh) << 16;
+  // rint((x - o) / d) - 16 by the reciprocal (off by less than 2^-17 here); within 2^-12 of a tie, by the division
+  const float rd = d > 0.f ? __frcp_rn(d) : 0.f;
+  float near = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = g.d > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[i], g.o), g.d)) - 16.0f : 0.f;
-    g.c[i] = (uint32_t)fminf(fmaxf(q, 0.f), 15.f);
+    const float y = fminf(fmaxf(fmaf(__fsub_rn(x[i], o), rd, -16.f), 0.f), 15.f), z = y + kMagic;
+    near = fmaxf(near, fabsf(y - (z - kMagic)));
+    g.c[i] = __float_as_uint(z);
+  }
+  if (near > 0.5f - 0x1p-12f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      g.c[i] = __float_as_uint(fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], o), d)) - 16.0f, 0.f), 15.f) + kMagic);
   }
   return g;
 }
-__device__ __forceinline__ uint16_t half_bits(float x) { return __half_as_ushort(__float2half_rn(x)); }
-
-// Which rows a group of hd / 8 lanes takes: of the packed rows 2 m and 2 m + 1 those that lead a token pair of
-// the cache (an even token, or the first row of a sequence), each with its partner when that is a row too.  A
-// pair's V codes share words, so a group that holds both tokens stores whole words.
-struct Lead {
-  int seq = -1, row, pos;
-  bool two;   // the partner pos + 1 is row + 1
-};
-__device__ __forceinline__ Lead lead_of(const ms_kv4_rows& r, int n_seqs, int j) {
-  Lead l;
-  if (j >= r.total) return l;
-  const int i = seq_of_row(r.cu, n_seqs, j);
-  if (i < 0) return l;
-  const int at = j - r.cu[i], pos = r.start[i] + at;
-  if ((pos & 1) && at > 0) return l;
-  l.seq = i;
-  l.row = j;
-  l.pos = pos;
-  l.two = !(pos & 1) && j + 1 < r.cu[i + 1] && j + 1 < r.total;
-  return l;
+// sum of c[i] << shift[i]; the magic parts of the c add up to a constant modulo 2^32
+__device__ __forceinline__ uint32_t k_word(const Group8& g) {
+  uint32_t w = 0, k = 0;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    w += g.c[2 * n] * (1u << (4 * n)) + g.c[2 * n + 1] * (1u << (4 * n + 16));
+    k += 0x4B400000u * (1u << (4 * n)) + 0x4B400000u * (1u << (4 * n + 16));
+  }
+  return w - k;
+}
+// four codes of one token and four of its partner, as the two halves of a word
+__device__ __forceinline__ uint32_t v_word(const uint32_t* a, const uint32_t* b) {
+  uint32_t w = 0, k = 0;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    w += a[n] * (1u << (4 * n)) + b[n] * (1u << (4 * n + 16));
+    k += 0x4B400000u * (1u << (4 * n)) + 0x4B400000u * (1u << (4 * n + 16));
+  }
+  return w - k;
 }
 
+// A row's heads are laid over the threads in order, 8 dims a thread, so a block's threads run through its rows.
 template <class T, int HD>
-__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const ms_kv4_cache c, const ms_kv4_rows r, uint32_t* err) {
+__global__ void __launch_bounds__(kThreads) kv4_write_kernel(const ms_kv4_cache c, const ms_kv4_rows r, int rows, uint32_t* err) {
   constexpr int LPR = HD / 8, G = HD / 32;
-  const int part = threadIdx.x % LPR, w = part >> 2, t = part & 3;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-  const int head = item % c.kv_heads;
-  const int64_t m = item / c.kv_heads;
-  for (int e = 0; e < 2; ++e) {
-    Lead l;
-    if (2 * m + e < r.total) l = lead_of(r, c.n_seqs, (int)(2 * m + e));
-    uint8_t* blk = l.seq >= 0 ? kv4_block(c, l.seq, l.pos, head) : nullptr;
-    if (l.seq >= 0 && !blk && part == 0) atomicOr(err, EF_BAD_INDEX);
-    Group8 k[2], v[2];
-    // every lane quantises (the shuffles need whole warps); lanes without a row work on zeros
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (blk && (p == 0 || l.two)) {
-        Raw8<T> a, b;
-        a.load((const T*)r.k + (int64_t)(l.row + p) * r.k_stride + head * HD + part * 8);
-        b.load((const T*)r.v + (int64_t)(l.row + p) * r.v_stride + head * HD + part * 8);
-        a.get(x);
-        b.get(y);
+  __shared__ Leads ls;
+  find_leads(c, r, rows, ls, err);
+  const int width = c.kv_heads * LPR, n = ls.n, per_head = c.page_tokens / 16;
+  int k = 0, at = threadIdx.x;
+  while (at >= width) { at -= width; ++k; }
+  for (int b = 0; b < n * width; b += kThreads) {          // the same count for all threads: the lanes exchange minima
+    const bool live = k < n;
+    const int tk = live ? ls.tok[k] : 0, row = live ? ls.row[k] : 0;
+    const bool two = tk & 16;
+    const int64_t at_k = (int64_t)row * r.k_stride + at * 8, at_v = (int64_t)row * r.v_stride + at * 8;
+    Raw8<T> kr[2], vr[2];
+    kr[0].zero(); kr[1].zero(); vr[0].zero(); vr[1].zero();
+    if (live) {
+      kr[0].load((const T*)r.k + at_k);
+      vr[0].load((const T*)r.v + at_v);
+      if (two) {
+        kr[1].load((const T*)r.k + at_k + r.k_stride);
+        vr[1].load((const T*)r.v + at_v + r.v_stride);
       }
-      k[p] = quantise8(x);
-      v[p] = quantise8(y);
     }
-    if (!blk) continue;
-    const int tok = l.pos & 15, pair = tok >> 1;
-    uint16_t vq[2][2];   // [token of the pair][quad]
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      if (p == 1 && !l.two) break;
-      uint32_t word = 0;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) word |= k[p].c[2 * n] << (4 * n) | k[p].c[2 * n + 1] << (4 * n + 16);
-      reinterpret_cast<uint32_t*>(blk)[(tok + p) * 4 * G + t * G + w] = word;
-      if (t == 0)
-        reinterpret_cast<uint32_t*>(blk + kv4_k_scales(HD))[(tok + p) * G + w] =
-            half_bits(k[p].d) | (uint32_t)half_bits(k[p].o) << 16;
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        vq[p][q] = (uint16_t)(v[p].c[4 * q] | v[p].c[4 * q + 1] << 4 | v[p].c[4 * q + 2] << 8 | v[p].c[4 * q + 3] << 12);
+    const int head = at / LPR, part = at % LPR, w = part >> 2, t = part & 3, tok = tk & 15, pair = tok >> 1;
+    uint8_t* blk = (uint8_t*)c.pages + ((live ? ls.block[k] : 0) + (int64_t)head * per_head) * kv4_block_bytes(HD);
+    uint32_t* ks = reinterpret_cast<uint32_t*>(blk + kv4_k_scales(HD)) + tok * G + w;
+    uint32_t* kc = reinterpret_cast<uint32_t*>(blk) + tok * 4 * G + t * G + w;
+    {
+      const Group8 g = quantise8(kr[0]);
+      if (live) {
+        *kc = k_word(g);
+        if (t == 0) *ks = g.scale;
+      }
     }
+    const bool any_two = __any_sync(0xffffffffu, two);
+    if (any_two) {
+      const Group8 g = quantise8(kr[1]);
+      if (live && two) {
+        kc[4 * G] = k_word(g);
+        if (t == 0) ks[G] = g.scale;
+      }
+    }
+    const Group8 g0 = quantise8(vr[0]);
     // lanes 2 C and 2 C + 1 hold the quads 0, 1 and 2, 3 of chunk C
     uint16_t* vc = reinterpret_cast<uint16_t*>(blk + kv4_v_codes(HD)) + (pair * (HD / 16) + kv4_v_chunk<HD>(part >> 1, pair)) * 8 + (part & 1) * 4;
     uint16_t* vs = reinterpret_cast<uint16_t*>(blk + kv4_v_scales(HD)) + (pair * G + w) * 4;
-    if (l.two) {
-      *reinterpret_cast<uint2*>(vc) = make_uint2(vq[0][0] | (uint32_t)vq[1][0] << 16, vq[0][1] | (uint32_t)vq[1][1] << 16);
-      if (t == 0)
-        *reinterpret_cast<uint2*>(vs) = make_uint2(half_bits(v[0].d) | (uint32_t)half_bits(v[1].d) << 16,
-                                                   half_bits(v[0].o) | (uint32_t)half_bits(v[1].o) << 16);
-    } else {
-      const int par = tok & 1;
-      vc[par] = vq[0][0];
-      vc[2 + par] = vq[0][1];
-      if (t == 0) {
-        vs[par] = half_bits(v[0].d);
-        vs[2 + par] = half_bits(v[0].o);
+    if (any_two) {
+      const Group8 g1 = quantise8(vr[1]);
+      if (live && two) {
+        *reinterpret_cast<uint2*>(vc) = make_uint2(v_word(g0.c, g1.c), v_word(g0.c + 4, g1.c + 4));
+        if (t == 0)
+          *reinterpret_cast<uint2*>(vs) = make_uint2(__byte_perm(g0.scale, g1.scale, 0x5410), __byte_perm(g0.scale, g1.scale, 0x7632));
       }
     }
+    if (live && !two) {
+      const int par = tok & 1;
+      vc[par] = (uint16_t)v_word(g0.c, g0.c);
+      vc[2 + par] = (uint16_t)v_word(g0.c + 4, g0.c + 4);
+      if (t == 0) {
+        vs[par] = (uint16_t)g0.scale;
+        vs[2 + par] = (uint16_t)(g0.scale >> 16);
+      }
+    }
+    at += kThreads;
+    while (at >= width) { at -= width; ++k; }
   }
 }
 
-// the 4 codes of a 16-bit quad -> values
-__device__ __forceinline__ void quad_values(uint32_t u, float d, float o, float* x) {
-#pragma unroll
-  for (int n = 0; n < 4; ++n) x[n] = fmaf(d, (float)(16 + ((u >> (4 * n)) & 15u)), o);   // d * (16 + c) is exact
+// nibble N of a word as the f32 number 16 + c: the code in the mantissa bits of 16 that weigh 1 to 8
+template <int N>
+__device__ __forceinline__ float code_f32(uint32_t w) {
+  constexpr int UP = 19 - 4 * N;
+  return __uint_as_float(((UP >= 0 ? w << (UP >= 0 ? UP : 0) : w >> (UP < 0 ? -UP : 0)) & 0x00780000u) | 0x41800000u);
+}
+// values o + d (16 + c) of 8 codes; d (16 + c) is exact
+__device__ __forceinline__ void k_values(uint32_t w, float d, float o, float (&x)[8]) {
+  x[0] = fmaf(d, code_f32<0>(w), o); x[1] = fmaf(d, code_f32<4>(w), o);
+  x[2] = fmaf(d, code_f32<1>(w), o); x[3] = fmaf(d, code_f32<5>(w), o);
+  x[4] = fmaf(d, code_f32<2>(w), o); x[5] = fmaf(d, code_f32<6>(w), o);
+  x[6] = fmaf(d, code_f32<3>(w), o); x[7] = fmaf(d, code_f32<7>(w), o);
+}
+template <int HALF>
+__device__ __forceinline__ void v_values(uint2 w, float d, float o, float (&x)[8]) {
+  constexpr int H = 4 * HALF;
+  x[0] = fmaf(d, code_f32<H>(w.x), o); x[1] = fmaf(d, code_f32<H + 1>(w.x), o);
+  x[2] = fmaf(d, code_f32<H + 2>(w.x), o); x[3] = fmaf(d, code_f32<H + 3>(w.x), o);
+  x[4] = fmaf(d, code_f32<H>(w.y), o); x[5] = fmaf(d, code_f32<H + 1>(w.y), o);
+  x[6] = fmaf(d, code_f32<H + 2>(w.y), o); x[7] = fmaf(d, code_f32<H + 3>(w.y), o);
 }
 
 template <class T, int HD>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const ms_kv4_cache c, const ms_kv4_rows r, uint32_t* err) {
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(const ms_kv4_cache c, const ms_kv4_rows r, int rows, uint32_t* err) {
   constexpr int LPR = HD / 8, G = HD / 32;
-  const int part = threadIdx.x % LPR, w = part >> 2, t = part & 3;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-  const int head = item % c.kv_heads;
-  const int64_t m = item / c.kv_heads;
-  for (int e = 0; e < 2; ++e) {
-    if (2 * m + e >= r.total) return;
-    const Lead l = lead_of(r, c.n_seqs, (int)(2 * m + e));
-    if (l.seq < 0) continue;
-    const uint8_t* blk = kv4_block(c, l.seq, l.pos, head);
-    if (!blk) {
-      if (part == 0) atomicOr(err, EF_BAD_INDEX);
-      continue;
-    }
-    const int tok = l.pos & 15, pair = tok >> 1;
+  __shared__ Leads ls;
+  find_leads(c, r, rows, ls, err);
+  const int width = c.kv_heads * LPR, n = ls.n, per_head = c.page_tokens / 16;
+  int k = 0, at = threadIdx.x;
+  while (at >= width) { at -= width; ++k; }
+#pragma unroll 2
+  for (; k < n;) {
+    const int tk = ls.tok[k], row = ls.row[k], head = at / LPR, part = at % LPR, w = part >> 2, t = part & 3, tok = tk & 15, pair = tok >> 1;
+    const uint8_t* blk = (const uint8_t*)c.pages + (ls.block[k] + (int64_t)head * per_head) * kv4_block_bytes(HD);
+    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk) + tok * 4 * G + t * G + w;
+    const uint32_t* ks = reinterpret_cast<const uint32_t*>(blk + kv4_k_scales(HD)) + tok * G + w;
+    const bool two = tk & 16;
+    const uint32_t k0 = kc[0], s0 = ks[0], k1 = two ? kc[4 * G] : 0u, s1 = two ? ks[G] : 0u;
     const uint2 vw = *reinterpret_cast<const uint2*>(blk + kv4_v_codes(HD) + (pair * (HD / 16) + kv4_v_chunk<HD>(part >> 1, pair)) * 16 + (part & 1) * 8);
     const uint2 vs = *reinterpret_cast<const uint2*>(blk + kv4_v_scales(HD) + (pair * G + w) * 8);
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      if (p == 1 && !l.two) break;
-      const uint32_t kw = reinterpret_cast<const uint32_t*>(blk)[(tok + p) * 4 * G + t * G + w];
-      const float2 ks = unpack2<__half>(reinterpret_cast<const uint32_t*>(blk + kv4_k_scales(HD))[(tok + p) * G + w]);
-      float x[8], y[8];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        x[2 * n] = fmaf(ks.x, (float)(16 + ((kw >> (4 * n)) & 15u)), ks.y);
-        x[2 * n + 1] = fmaf(ks.x, (float)(16 + ((kw >> (4 * n + 16)) & 15u)), ks.y);
-      }
-      const int sh = ((tok + p) & 1) * 16;
-      const float vd = h2f_bits((uint16_t)(vs.x >> sh)), vo = h2f_bits((uint16_t)(vs.y >> sh));
-      quad_values((vw.x >> sh) & 0xFFFFu, vd, vo, y);
-      quad_values((vw.y >> sh) & 0xFFFFu, vd, vo, y + 4);
-      store8((T*)r.k + (int64_t)(l.row + p) * r.k_stride + head * HD + part * 8, x);
-      store8((T*)r.v + (int64_t)(l.row + p) * r.v_stride + head * HD + part * 8, y);
+    T* kd = (T*)r.k + (int64_t)row * r.k_stride + at * 8;
+    T* vd = (T*)r.v + (int64_t)row * r.v_stride + at * 8;
+    const float2 vds = unpack2<__half>(vs.x), vos = unpack2<__half>(vs.y);
+    float x[8];
+    float2 s = unpack2<__half>(s0);
+    k_values(k0, s.x, s.y, x);
+    store8(kd, x);
+    if (tok & 1) v_values<1>(vw, vds.y, vos.y, x);
+    else v_values<0>(vw, vds.x, vos.x, x);
+    store8(vd, x);
+    if (two) {
+      s = unpack2<__half>(s1);
+      k_values(k1, s.x, s.y, x);
+      store8(kd + r.k_stride, x);
+      v_values<1>(vw, vds.y, vos.y, x);
+      store8(vd + r.v_stride, x);
     }
+    at += kThreads;
+    while (at >= width) { at -= width; ++k; }
   }
 }
 
 template <class T, int HD>
 cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_rows& r, bool write, cudaStream_t s) {
-  const int64_t items = ((int64_t)r.total + 1) / 2 * c.kv_heads, per = kThreads / (HD / 8);
-  const uint32_t grid = (uint32_t)((items + per - 1) / per);
-  if (write) kv4_write_kernel<T, HD><<<grid, kThreads, 0, s>>>(c, r, d.err);
-  else kv4_read_kernel<T, HD><<<grid, kThreads, 0, s>>>(c, r, d.err);
+  // 16 rows share a look-up; with few of them 2, so that a decode step spreads over the SMs
+  int rows = kRows;
+  while (rows > 2 && (int64_t)r.total < (int64_t)rows * 4 * d.sm_count) rows /= 2;
+  const uint32_t grid = (uint32_t)(((int64_t)r.total + rows - 1) / rows);
+  if (write) kv4_write_kernel<T, HD><<<grid, kThreads, 0, s>>>(c, r, rows, d.err);
+  else kv4_read_kernel<T, HD><<<grid, kThreads, 0, s>>>(c, r, rows, d.err);
   return cudaGetLastError();
 }
 

@@ -19,15 +19,15 @@ __device__ __forceinline__ int kv4_v_chunk(int C, int pair) {
   return HD == 64 ? C ^ (pair & 2) : C ^ ((pair & 3) << 1);
 }
 
-// the block of token pos of a sequence, or null where position or page number are outside their tables
-__device__ __forceinline__ uint8_t* kv4_block(const ms_kv4_cache& c, int seq, int pos, int head) {
-  if (pos < 0) return nullptr;
+// the block of token pos of a sequence, counted in blocks from the start of the pages, or -1 where position or page
+// number are outside their tables
+__device__ __forceinline__ int64_t kv4_block(const ms_kv4_cache& c, int seq, int pos, int head) {
+  if (pos < 0) return -1;
   const int j = pos / c.page_tokens;
-  if (j >= c.max_pages) return nullptr;
+  if (j >= c.max_pages) return -1;
   const int page = c.block_table[(int64_t)seq * c.max_pages + j];
-  if (page < 0 || page >= c.n_pages) return nullptr;
-  const int64_t blk = ((int64_t)page * c.kv_heads + head) * (c.page_tokens / 16) + (pos % c.page_tokens) / 16;
-  return (uint8_t*)c.pages + blk * kv4_block_bytes(c.head_dim);
+  if (page < 0 || page >= c.n_pages) return -1;
+  return ((int64_t)page * c.kv_heads + head) * (c.page_tokens / 16) + (pos % c.page_tokens) / 16;
 }
 
 }  // namespace ms
