@@ -32,10 +32,21 @@ __device__ __forceinline__ void find_leads(const ms_kv4_cache& c, const ms_kv4_r
     bool lead = false;
     int64_t block = 0;
     int tok = 0;
+    // the row's sequence: up to 32 sequences from one load, more by bisection
+    int i = -1, begin = 0, end = 0, first = 0;
+    if (c.n_seqs <= 32) {
+      const int lo = lane < c.n_seqs ? r.cu[lane] : 0x7fffffff, hi = lane < c.n_seqs ? r.cu[lane + 1] : 0, st = lane < c.n_seqs ? r.start[lane] : 0;
+      for (int s = 0; s < c.n_seqs; ++s) {
+        const int l = __shfl_sync(0xffffffffu, lo, s), h = __shfl_sync(0xffffffffu, hi, s), f = __shfl_sync(0xffffffffu, st, s);
+        if (l <= j && j < h) { i = s; begin = l; end = h; first = f; }
+      }
+    } else if (j < r.total) {
+      i = seq_of_row(r.cu, c.n_seqs, j);
+      if (i >= 0) { begin = r.cu[i]; end = r.cu[i + 1]; first = r.start[i]; }
+    }
     if (lane < rows && j < r.total) {
-      const int i = seq_of_row(r.cu, c.n_seqs, j);
       if (i >= 0) {
-        const int begin = r.cu[i], end = r.cu[i + 1], at = j - begin, pos = r.start[i] + at;
+        const int at = j - begin, pos = first + at;
         if (!(pos & 1) || at == 0) {
           block = kv4_block(c, i, pos, 0);
           lead = block >= 0;
