@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const ms_qk_rope a, u
     }
   }
   constexpr int HD = LPR * 16;
+  const unsigned mask = (LPR == 32 ? 0xffffffffu : (1u << LPR) - 1) << (threadIdx.x % 32 / LPR * LPR);   // the lanes of the head
   const int half = a.rot_dim / 2;
   const bool turns = 16 * lane < a.rot_dim;
   const int d0 = !INTER && turns ? 8 * lane : 16 * lane, d1 = !INTER && turns ? d0 + half : d0 + 8;
@@ -49,53 +50,57 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const ms_qk_rope a, u
       r[i][0].load(src + (h0 + i) * HD + d0);
       r[i][1].load(src + (h0 + i) * HD + d1);
     }
-  float cs[8], sn[8], w[16];
-  if (live && turns) {   // 8 pairs per lane: (8 l + i, half + 8 l + i), or 2 i and 2 i + 1 of its 16 dims
+  // 8 pairs per lane, (8 l + i, half + 8 l + i) or 2 i and 2 i + 1 of its 16 dims, and the 16 weights
+  float4 cs[2], sn[2], w[4];
+  if (live && turns) {
     const float4* c4 = reinterpret_cast<const float4*>(a.cos_t + (int64_t)pos * half + 8 * lane);
     const float4* s4 = reinterpret_cast<const float4*>(a.sin_t + (int64_t)pos * half + 8 * lane);
-    *reinterpret_cast<float4*>(cs) = c4[0]; *reinterpret_cast<float4*>(cs + 4) = c4[1];
-    *reinterpret_cast<float4*>(sn) = s4[0]; *reinterpret_cast<float4*>(sn + 4) = s4[1];
+    cs[0] = c4[0]; cs[1] = c4[1];
+    sn[0] = s4[0]; sn[1] = s4[1];
   }
   const float* nw = is_q ? a.q_norm : a.k_norm;
   if (nw) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { w[i] = nw[d0 + i]; w[8 + i] = nw[d1 + i]; }
+    w[0] = reinterpret_cast<const float4*>(nw + d0)[0]; w[1] = reinterpret_cast<const float4*>(nw + d0)[1];
+    w[2] = reinterpret_cast<const float4*>(nw + d1)[0]; w[3] = reinterpret_cast<const float4*>(nw + d1)[1];
   }
+  const float *c = reinterpret_cast<const float*>(cs), *s = reinterpret_cast<const float*>(sn), *ww = reinterpret_cast<const float*>(w);
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
+    if (h0 + i >= nh) break;             // the same for the lanes of a head
     float x[2][8];
     r[i][0].get(x[0]);
     r[i][1].get(x[1]);
     if (nw) {
-      float ss = 0.f;
+      float ss[2] = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(x[0][j], x[0][j], fmaf(x[1][j], x[1][j], ss));
+      for (int j = 0; j < 8; ++j) { ss[0] = fmaf(x[0][j], x[0][j], ss[0]); ss[1] = fmaf(x[1][j], x[1][j], ss[1]); }
+      float sum = ss[0] + ss[1];
 #pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float inv = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
+      for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+      const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);   // within 2^-22 of the root's reciprocal
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { x[0][j] *= inv * w[j]; x[1][j] *= inv * w[8 + j]; }
+      for (int j = 0; j < 8; ++j) { x[0][j] = x[0][j] * inv * ww[j]; x[1][j] = x[1][j] * inv * ww[8 + j]; }
     }
     if (turns) {
       if (INTER) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float u = x[c][2 * j], v = x[c][2 * j + 1], co = cs[4 * c + j], si = sn[4 * c + j];
-            x[c][2 * j] = u * co - v * si;
-            x[c][2 * j + 1] = v * co + u * si;
+            const float u = x[q][2 * j], v = x[q][2 * j + 1], co = c[4 * q + j], si = s[4 * q + j];
+            x[q][2 * j] = u * co - v * si;
+            x[q][2 * j + 1] = v * co + u * si;
           }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float u = x[0][j], v = x[1][j];
-          x[0][j] = u * cs[j] - v * sn[j];
-          x[1][j] = v * cs[j] + u * sn[j];
+          x[0][j] = u * c[j] - v * s[j];
+          x[1][j] = v * c[j] + u * s[j];
         }
       }
     }
-    if (live && h0 + i < nh) {
+    if (live) {
       store8(dst + (h0 + i) * HD + d0, x[0]);
       store8(dst + (h0 + i) * HD + d1, x[1]);
     }
@@ -159,7 +164,8 @@ void start(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
   const int hd = a.head_dim;
   const bool vec = (hd == 64 || hd == 128 || hd == 256) && a.rot_dim % 16 == 0 && a.q_stride % 8 == 0 &&
                    a.k_stride % 8 == 0 && a.q_out_stride % 8 == 0 && a.k_out_stride % 8 == 0 && aligned16(a.q) &&
-                   aligned16(a.k) && aligned16(a.q_out) && aligned16(a.k_out) && aligned16(a.cos_t) && aligned16(a.sin_t);
+                   aligned16(a.k) && aligned16(a.q_out) && aligned16(a.k_out) && aligned16(a.cos_t) && aligned16(a.sin_t) &&
+                   aligned16(a.q_norm) && aligned16(a.k_norm);
   if (!vec) {
     const uint64_t items = (uint64_t)a.n_tokens * (a.heads + a.kv_heads);
     qk_rope_any_kernel<TI, TO><<<(uint32_t)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, s>>>(a, c.err);
