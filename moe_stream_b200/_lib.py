@@ -148,13 +148,13 @@ _SIGS = {
     "ms_model_router_stats": (C.c_int, [_vp, _fp, _ip]),
     "ms_model_router_totals": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i, C.POINTER(C.c_int)]),
     "ms_model_expert_tier_stats": (C.c_int, [_vp, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
-    "ms_qk_norm_rope": (C.c_int, [_vp, C.POINTER(QkRope)]),
-    "ms_prompt_attention": (C.c_int, [_vp, C.POINTER(PromptAttn)]),
+    "ms_qk_norm_rope": (C.c_int, [_vp, _vp]),
+    "ms_prompt_attention": (C.c_int, [_vp, _vp]),
     "ms_kv4_page_bytes": (C.c_int, [_i, _i, _i, C.POINTER(C.c_size_t)]),
-    "ms_kv4_write": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows)]),
-    "ms_kv4_read": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Rows)]),
-    "ms_kv4_attention_workspace": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), _i, _i, C.POINTER(C.c_size_t)]),
-    "ms_kv4_attention": (C.c_int, [_vp, C.POINTER(Kv4CacheArgs), C.POINTER(Kv4Attn)]),
+    "ms_kv4_write": (C.c_int, [_vp, _vp, _vp]),
+    "ms_kv4_read": (C.c_int, [_vp, _vp, _vp]),
+    "ms_kv4_attention_workspace": (C.c_int, [_vp, _vp, _i, _i, C.POINTER(C.c_size_t)]),
+    "ms_kv4_attention": (C.c_int, [_vp, _vp, _vp]),
     "ms_model_get_config": (C.c_int, [_vp, C.POINTER(ModelConfig)]),
     "ms_model_destroy": (C.c_int, [_vp]),
     "ms_model_forward": (C.c_int, [_vp, _ip, _i, _fp]),
