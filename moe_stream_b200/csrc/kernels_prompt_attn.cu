@@ -35,21 +35,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;   // the running maximum before any key
 constexpr float kRaise = 4096.f;  // sum of a row's probabilities of a tile that raises the running maximum
 
-template <int HD>
+// CL: blocks that share an MMA (a pair reads each K and V tile once for twice the rows, half of it each)
+template <int HD, int CL>
 struct Shape {
   static constexpr int NQ = HD == 256 ? 1 : 2;          // query tiles of a block
-  static constexpr int BN = HD == 256 ? 64 : 128;       // keys of a tile
-  static constexpr int STAGES = HD == 64 ? 4 : HD == 128 ? 2 : 3;   // of K and of V
-  static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = BN * HD * 2;
-  static constexpr int SOFTMAX_WARPS = 4 * NQ, THREADS = 32 * (SOFTMAX_WARPS + (NQ == 2 ? 4 : 2));
-  // NQ = 1: queries in tensor memory and probabilities in shared memory, so that the score product, whose tiles are
-  // half as wide, reads one operand from shared memory only (both would need 192 bytes a cycle of its 128)
-  static constexpr int P_BYTES = NQ == 1 ? 128 * BN * 2 : 0;
-  static constexpr int SMEM = 1024 + (NQ == 2 ? NQ * Q_BYTES : 2 * P_BYTES) + 2 * STAGES * KV_BYTES;
-  // columns of tensor memory: two score buffers, the outputs; then with 64 dims the probabilities of the two buffers
-  // (with 128 dims, which fill all 512 columns, they take the first half of the scores they came from), with 256
-  // dims the queries
-  static constexpr uint32_t O_COL = 2 * BN, P_COL = HD == 128 ? 0 : O_COL + NQ * HD, P_STEP = HD == 128 ? BN : BN / 2, Q_COL = O_COL + HD;
+  static constexpr int BN = 128;                        // keys of a tile
+  static constexpr int STAGES = HD == 64 ? 4 : 2 * (HD == 256 ? 1 : CL);   // of K and of V
+  static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = BN * HD * 2 / CL;
+  static constexpr int K_ROWS = BN / CL, V_BLOCKS = HD / 64 / CL;   // a block's share: rows of K, blocks of 64 dims of V
+  static constexpr int SOFTMAX_WARPS = 4 * NQ, THREADS = 32 * (SOFTMAX_WARPS + 4);
+  static constexpr int SMEM = 1024 + NQ * Q_BYTES + 2 * STAGES * KV_BYTES;
+  // columns of tensor memory: two score buffers, the outputs and, with 64 dims, the probabilities of the two buffers;
+  // otherwise all 512 columns are full and the probabilities take the first half of the scores they came from
+  static constexpr uint32_t O_COL = 2 * BN, P_COL = HD == 64 ? O_COL + NQ * HD : 0, P_STEP = HD == 64 ? BN / 2 : BN;
   static constexpr uint32_t COLS = 512;
 };
 
@@ -99,10 +97,10 @@ struct Place {
   int tiles, first;          // key tiles, and the first one's index in the sequence
   bool ok;
 };
-template <int HD>
+template <int HD, int CL>
 __device__ __forceinline__ Place find_place(const ms_prompt_attn& a, int n_tok, int index, uint32_t* err) {
-  using S = Shape<HD>;
-  const int lane = threadIdx.x & 31, per = S::NQ * n_tok;
+  using S = Shape<HD, CL>;
+  const int lane = threadIdx.x & 31, per = CL * S::NQ * n_tok;
   Place p;
   p.ok = false;
   // blocks of all sequences; this one counts from the last, so that the longest rows of a prompt start first
@@ -148,98 +146,150 @@ __device__ __forceinline__ Place find_place(const ms_prompt_attn& a, int n_tok, 
   return p;
 }
 
-template <class T, int HD>
-__global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
+// ---- between the blocks of a pair ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+// Arrive on the same mbarrier of the block with rank 0.  What the arrival stands for was done by TMA or is in tensor
+// memory (ordered by tcgen05.fence), so it needs no release of ordinary memory at cluster scope, which costs about a
+// thousand cycles; the one place where it stands for ordinary stores fences by itself.
+__device__ __forceinline__ void arrive_at_first(uint64_t* bar) {
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+template <class T, int HD, int CL>
+__global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
     prompt_attn_kernel(const ms_prompt_attn a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map, int n_tok, uint32_t* err) {
-  using S = Shape<HD>;
+  using S = Shape<HD, CL>;
   constexpr int NQ = S::NQ, BN = S::BN, ST = S::STAGES, BLK = HD / 64;   // BLK: blocks of 64 dims
   constexpr bool BF16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *sq = sm, *sk = sq + (NQ == 2 ? NQ * S::Q_BYTES : 2 * S::P_BYTES), *sv = sk + ST * S::KV_BYTES;   // NQ = 1: sq holds probabilities
-  __shared__ uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[NQ];
+  uint8_t *sq = sm, *sk = sq + NQ * S::Q_BYTES, *sv = sk + ST * S::KV_BYTES;
+  // *_other (rank 0 of a pair): the other block's share has arrived, too
+  __shared__ uint64_t q_full, q_other, k_full[ST], k_other[ST], k_empty[ST], v_full[ST], v_other[ST], v_empty[ST], s_full[2], p_full[2],
+      o_full[NQ];
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.x % a.kv_heads, rep = a.heads / a.kv_heads;
-  const Place pl = find_place<HD>(a, n_tok, blockIdx.x / a.kv_heads, err);
-  if (!pl.ok) return;
+  const int rank = CL == 2 ? cluster_rank() : 0, index = blockIdx.x / CL;
+  const int head = index % a.kv_heads, rep = a.heads / a.kv_heads;
+  const Place pl = find_place<HD, CL>(a, n_tok, index / a.kv_heads, err);
+  if (!pl.ok) return;                      // both blocks of a pair
 
-  if (warp == S::SOFTMAX_WARPS) {
-    umma::tmem_alloc(&tmem_base, S::COLS);
-    umma::tmem_relinquish();
-  }
+  if (warp == S::SOFTMAX_WARPS) umma::alloc_cg<CL>(&tmem_base, S::COLS);
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, NQ == 2 ? 1 : 4);
+    mbar_init(&q_full, 1);
+    mbar_init(&q_other, 1);
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+      mbar_init(&k_full[i], 1); mbar_init(&k_other[i], 1); mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1); mbar_init(&v_other[i], 1); mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4 * CL); }
     for (int i = 0; i < NQ; ++i) mbar_init(&o_full[i], 1);
     fence_mbar_init();
   }
   umma::fence_before_sync();
   __syncthreads();
+  if (CL == 2) cluster_sync();
   umma::fence_after_sync();
   constexpr uint32_t tmem = 0;             // all 512 columns are this block's, so they start at 0
   if (threadIdx.x == 0 && tmem_base != tmem) atomicOr(err, EF_BAD_SHAPE);
   const int nq = pl.q1 - pl.q0, nk = pl.k1 - pl.k0;
-  const int slots = NQ == 2 && pl.t0 + n_tok < nq ? 2 : 1;   // query tiles with rows
+  // query tile i of this block begins at token t0 + (i CL + rank) n_tok; slots: tiles with rows in any of the blocks
+  const int slots = NQ == 2 && pl.t0 + CL * n_tok < nq ? 2 : 1;
 
   // the two softmax groups need more than the 168 registers of 384 threads: 208 x 256 + 80 x 128 of 168 x 384
   if (warp >= S::SOFTMAX_WARPS) {
     if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == S::SOFTMAX_WARPS + 1) {
-      // ---- TMA ----
+    // (a wait that runs out does so for the whole warp)
+    auto wait = [&](uint64_t* bar, int parity) {
+      return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
+    };
+    // rows of V behind the sequence's end are rows of others: zeroed (16-byte units of 128-byte rows)
+    auto clear_tail = [&](int j) {
+      const int keys = nk - (pl.first + j) * BN, bad = BN - keys;
+      if (bad <= 0) return false;
+      for (int i = lane; i < bad * 8 * S::V_BLOCKS; i += 32) {
+        const int b = i / (bad * 8), u = i % (bad * 8);
+        *reinterpret_cast<uint4*>(sv + j % ST * S::KV_BYTES + b * BN * 128 + keys * 128 + u * 16) = make_uint4(0, 0, 0, 0);
+      }
+      umma::fence_proxy_async_smem();
+      __syncwarp();
+      return true;
+    };
+    // the first of the four warps issues the MMAs, the next two the copies of K and of V; in the other block of a pair the
+    // first and the last tell the first block what has arrived
+    const int role = warp - S::SOFTMAX_WARPS;
+    if (role == 1 || role == 2) {
+      // ---- TMA: Q and K, or V ----
       if (lane == 0 && pl.tiles > 0) {
-        const int rows = n_tok * rep;
-        if (NQ == 2) {
+        uint64_t *full = role == 1 ? k_full : v_full, *empty = role == 1 ? k_empty : v_empty;
+        if (role == 1) {
+          const int rows = n_tok * rep;
           mbar_expect_tx(&q_full, slots * BLK * rows * 128);
           for (int i = 0; i < slots; ++i)
             for (int b = 0; b < BLK; ++b)
-              tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + i * n_tok, &q_full);
+              tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + (i * CL + rank) * n_tok, &q_full);
         }
         bool alive = true;
-        for (int j = 0; j < pl.tiles && alive; ++j) {
+        for (int j = 0; j < pl.tiles; ++j) {
           const int st = j % ST, z = pl.k0 + (pl.first + j) * BN;
-          if (j >= ST) alive = mbar_wait(&k_empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY);
+          if (j >= ST) alive = mbar_wait(&empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY);
           if (!alive) break;
-          mbar_expect_tx(&k_full[st], S::KV_BYTES);
-          for (int b = 0; b < BLK; ++b) tma_3d(sk + st * S::KV_BYTES + b * BN * 128, &k_map, 64 * b, head, z, &k_full[st]);
-          if (j >= ST) alive = mbar_wait(&v_empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY);
-          if (!alive) break;
-          mbar_expect_tx(&v_full[st], S::KV_BYTES);
-          for (int b = 0; b < BLK; ++b) tma_3d(sv + st * S::KV_BYTES + b * BN * 128, &v_map, 64 * b, head, z, &v_full[st]);
+          mbar_expect_tx(&full[st], S::KV_BYTES);
+          if (role == 1) {
+            for (int b = 0; b < BLK; ++b)
+              tma_3d(sk + st * S::KV_BYTES + b * S::K_ROWS * 128, &k_map, 64 * b, head, z + rank * S::K_ROWS, &full[st]);
+          } else {
+            for (int b = 0; b < S::V_BLOCKS; ++b)
+              tma_3d(sv + st * S::KV_BYTES + b * BN * 128, &v_map, 64 * (rank * S::V_BLOCKS + b), head, z, &full[st]);
+          }
         }
         // nothing of this block may still be on its way when it ends (the copies of an unfinished walk, too)
         if (!alive) {
-          if (NQ == 2) mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
-          for (int i = 0; i < ST; ++i) { mbar_wait(&k_full[i], 0, nullptr, 0); mbar_wait(&v_full[i], 0, nullptr, 0); }
+          if (role == 1) mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
+          for (int i = 0; i < ST; ++i) mbar_wait(&full[i], 0, nullptr, 0);
         }
       }
-    } else if (warp == S::SOFTMAX_WARPS) {
-      // ---- MMA: the whole warp walks, lane 0 issues ----
-      constexpr uint32_t id_s = umma::idesc_f16(128, BN, BF16, false), id_o = umma::idesc_f16(128, HD, BF16, true);
+    } else if (rank == 1) {
+      // ---- the other block of a pair: Q and K, or V ----
+      bool alive = pl.tiles > 0;
+      if (alive && role == 0) {
+        alive = wait(&q_full, 0);
+        if (alive && lane == 0) arrive_at_first(&q_other);
+      }
+      for (int j = 0; j < pl.tiles && alive; ++j) {
+        alive = wait(role == 0 ? &k_full[j % ST] : &v_full[j % ST], j / ST);
+        if (!alive) break;
+        if (role == 3 && clear_tail(j)) fence_cluster();
+        if (lane == 0) arrive_at_first(role == 0 ? &k_other[j % ST] : &v_other[j % ST]);
+      }
+    } else if (role == 0) {
+      // ---- MMA: the whole warp walks, one thread issues ----
+      constexpr uint32_t id_s = umma::idesc_f16(128 * CL, BN, BF16, false), id_o = umma::idesc_f16(128 * CL, HD, BF16, true);
       // descriptors of the first tiles; others are that many 16-byte units further
       const uint64_t dq = umma::smem_desc_sw128(sq, 0), dk = umma::smem_desc_sw128(sk, 0), dv = umma::smem_desc_sw128(sv, BN * 128);
       const bool one = umma::elect();
       auto free_stage = [&](uint64_t* bar, int j) {          // only where a copy waits for it: none is left open at the end
-        if (one && j + ST < pl.tiles) umma::commit(bar);
+        if (one && j + ST < pl.tiles) umma::commit_cg<CL>(bar);
         __syncwarp();
       };
-      // (a wait that runs out does so for the whole warp)
-      auto wait = [&](uint64_t* bar, int parity) {
-        return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
-      };
-      bool alive = pl.tiles > 0 && wait(&q_full, 0);
+      bool alive = pl.tiles > 0 && wait(&q_full, 0) && (CL == 1 || wait(&q_other, 0));
       // slot is a constant: its addresses are, too (a block issues an MMA every 64 cycles)
       auto scores = [&](auto slot_c, int j) {
         constexpr int slot = decltype(slot_c)::value;
         if (!alive || j >= pl.tiles) return;
         const int st = j % ST;
         if (NQ == 1 || slot == 0) {
-          alive = wait(&k_full[st], j / ST);
+          alive = wait(&k_full[st], j / ST) && (CL == 1 || wait(&k_other[st], j / ST));
           if (!alive) return;
           umma::fence_after_sync();
         }
@@ -249,12 +299,9 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
 #pragma unroll
             for (int b = 0; b < BLK; ++b)
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {
-                const uint64_t kd = k + (b * BN * 128 + kk * 32) / 16;
-                if (NQ == 2) umma::mma_bf16(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, kd, id_s, b || kk);
-                else umma::mma_f16_ts(slot * BN, S::Q_COL + (b * 4 + kk) * 8, kd, id_s, b || kk);
-              }
-            umma::commit(&s_full[slot]);
+              for (int kk = 0; kk < 4; ++kk)
+                umma::mma_ss<CL>(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, k + (b * S::K_ROWS * 128 + kk * 32) / 16, id_s, b || kk);
+            umma::commit_cg<CL>(&s_full[slot]);
           }
           __syncwarp();
         }
@@ -265,31 +312,22 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
         if (!alive || j >= pl.tiles) return;
         const int st = j % ST;
         if (NQ == 1 || slot == 0) {
-          alive = wait(&v_full[st], j / ST);
+          alive = wait(&v_full[st], j / ST) && (CL == 1 || wait(&v_other[st], j / ST));
           if (!alive) return;
-          const int keys = nk - (pl.first + j) * BN;           // keys of the sequence in this tile
-          if (keys < BN) {                                     // the rest are rows of others: zeroed (16-byte units of 128-byte rows)
-            for (int i = lane; i < (BN - keys) * 8 * BLK; i += 32) {
-              const int b = i / ((BN - keys) * 8), u = i % ((BN - keys) * 8);
-              *reinterpret_cast<uint4*>(sv + st * S::KV_BYTES + b * BN * 128 + keys * 128 + u * 16) = make_uint4(0, 0, 0, 0);
-            }
-            umma::fence_proxy_async_smem();
-            __syncwarp();
-          }
+          if (clear_tail(j) && CL == 2) fence_cluster();
         }
         if (NQ == 1 || slot < slots) {
-          alive = wait(&p_full[slot], NQ == 2 ? j : j >> 1);   // how often this buffer was filled before
+          const int turn = NQ == 2 ? j : j >> 1;               // how often this buffer was filled before
+          alive = wait(&p_full[slot], turn);
           if (!alive) return;
           umma::fence_after_sync();
           if (one) {
             const uint64_t v = dv + st * (S::KV_BYTES >> 4);
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk) {
-              const uint64_t vd = v + kk * 2048 / 16;
-              if (NQ == 2) umma::mma_f16_ts(S::O_COL + slot * HD, S::P_COL + slot * S::P_STEP + kk * 8, vd, id_o, j > 0 || kk > 0);
-              else umma::mma_bf16(S::O_COL, dq + slot * (S::P_BYTES >> 4) + kk * 32 / 16, vd, id_o, j > 0 || kk > 0);
-            }
-            umma::commit(&o_full[NQ == 2 ? slot : 0]);
+            for (int kk = 0; kk < BN / 16; ++kk)
+              umma::mma_ts<CL>(S::O_COL + (NQ == 2 ? slot * HD : 0), S::P_COL + slot * S::P_STEP + kk * 8, v + kk * 2048 / 16, id_o,
+                               j > 0 || kk > 0);
+            umma::commit_cg<CL>(&o_full[NQ == 2 ? slot : 0]);
           }
           __syncwarp();
         }
@@ -311,7 +349,7 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
     // ---- softmax: thread = row ----
     if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int tile = warp >> 2, r = threadIdx.x & 127;       // query tile of the block, row of it
-    const int tok = pl.t0 + tile * n_tok + r / rep;          // token of the sequence
+    const int tok = pl.t0 + (tile * CL + rank) * n_tok + r / rep;   // token of the sequence
     const bool row_ok = r < n_tok * rep && tok < nq;
     const int h = head * rep + r % rep;
     const int last = row_ok ? nk - nq + tok : -1;            // the row's last key
@@ -324,23 +362,6 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
     auto wait = [&](uint64_t* bar, int parity) {
       return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity & 1, err, EF_TIMEOUT_FULL));
     };
-    if (NQ == 1 && pl.tiles > 0) {       // the row's queries to tensor memory, as they are
-      const uint4* src = reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)(pl.q0 + tok) * a.q_stride + h * HD);
-#pragma unroll
-      for (int i = 0; i < HD / 64; ++i) {
-        uint32_t x[32];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint4 w = row_ok ? src[8 * i + e] : make_uint4(0, 0, 0, 0);
-          x[4 * e] = w.x; x[4 * e + 1] = w.y; x[4 * e + 2] = w.z; x[4 * e + 3] = w.w;
-        }
-        umma::st_32x32b_x32(tmem + lanes + S::Q_COL + 32 * i, x);
-      }
-      umma::wait_st();
-      umma::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
-    }
     if (tile < slots) {
       for (int j = 0; j < pl.tiles; ++j) {
         const int slot = NQ == 2 ? tile : j & 1, turn = NQ == 2 ? j : j >> 1;
@@ -414,20 +435,15 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
           }
         }
         l += sum;
-        if (NQ == 2) {
 #pragma unroll
-          for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(p_col + 32 * i, u + 32 * i);
-        } else {                                             // a row of 64 keys is 128 bytes, 16-byte units permuted as TMA would
-          uint8_t* dst = sq + slot * S::P_BYTES + r * 128;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(dst + ((i ^ (r & 7)) << 4)) = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
-          umma::fence_proxy_async_smem();
-        }
+        for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(p_col + 32 * i, u + 32 * i);
         umma::wait_st();
         umma::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[slot]);
+        if (lane == 0) {
+          if (CL == 1) mbar_arrive(&p_full[slot]);
+          else arrive_at_first(&p_full[slot]);
+        }
       }
       // ---- output ----
       // A wait on a phase's parity tells it from the one before only: the scores of tile j vouch for the value products
@@ -469,8 +485,9 @@ __global__ void __launch_bounds__(Shape<HD>::THREADS, 1)
   }
   umma::fence_before_sync();
   __syncthreads();
+  if (CL == 2) cluster_sync();             // no arrival may find a block that has ended
   umma::fence_after_sync();
-  if (warp == S::SOFTMAX_WARPS) umma::tmem_dealloc(tmem, S::COLS);
+  if (warp == S::SOFTMAX_WARPS) umma::dealloc_cg<CL>(tmem, S::COLS);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -498,31 +515,41 @@ bool make_map(CUtensorMap* map, bool bf16, const void* p, int hd, int heads, int
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int HD>
+template <class T, int HD, int CL>
 cudaError_t start(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
-  using S = Shape<HD>;
+  using S = Shape<HD, CL>;
   const int rep = a.heads / a.kv_heads, n_tok = 128 / rep;
   const bool bf16 = a.type == MS_Q_BF16;
   if (!encoder()) return cudaErrorNotSupported;
   CUtensorMap q, k, v;
   if (!make_map(&q, bf16, a.q, HD, a.heads, a.total_q, a.q_stride, rep, n_tok)) return cudaErrorInvalidValue;
   if (a.total_k == 0) k = v = q;   // no block has a key tile
-  else if (!make_map(&k, bf16, a.k, HD, a.kv_heads, a.total_k, a.k_stride, 1, S::BN) ||
+  else if (!make_map(&k, bf16, a.k, HD, a.kv_heads, a.total_k, a.k_stride, 1, S::K_ROWS) ||
            !make_map(&v, bf16, a.v, HD, a.kv_heads, a.total_k, a.v_stride, 1, S::BN))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(prompt_attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(prompt_attn_kernel<T, HD, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return e;
-  // blocks of all sequences: at most one that is not full for each
-  const int64_t blocks = ((int64_t)a.total_q / (S::NQ * n_tok) + a.n_seqs) * a.kv_heads;
-  prompt_attn_kernel<T, HD><<<(unsigned)blocks, S::THREADS, S::SMEM, s>>>(a, q, k, v, n_tok, d.err);
-  return cudaGetLastError();
+  // blocks (pairs) of all sequences: at most one that is not full for each
+  const int64_t places = ((int64_t)a.total_q / (CL * S::NQ * n_tok) + a.n_seqs) * a.kv_heads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(places * CL));
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CL;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CL == 2 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, prompt_attn_kernel<T, HD, CL>, a, q, k, v, n_tok, d.err);
 }
 
 template <class T>
 cudaError_t start_hd(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
-  if (a.head_dim == 64) return start<T, 64>(d, a, s);
-  if (a.head_dim == 128) return start<T, 128>(d, a, s);
-  return start<T, 256>(d, a, s);
+  if (a.head_dim == 64) return start<T, 64, 1>(d, a, s);
+  if (a.head_dim == 128) return start<T, 128, 1>(d, a, s);
+  return start<T, 256, 2>(d, a, s);
 }
 
 }  // namespace

@@ -153,14 +153,60 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool b
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (uint32_t)(N >> 3) << 17 |
          (uint32_t)(M >> 4) << 24;
 }
-// D[tmem] (+)= A x B^T, A in tensor memory: lane = row, one 32-bit column = two elements of K
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
-      : "memory");
+// ---- one block (CG = 1) or a pair of blocks of a cluster (CG = 2) on one MMA.  A pair computes M = 256: each block
+// holds 128 rows of A and of D and half of the rows of B, at the same addresses; one thread of the block with
+// rank 0 issues for both.  A kernel uses one CG throughout. ----
+template <int CG>
+__device__ __forceinline__ void alloc_cg(uint32_t* smem_dst, uint32_t ncols) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(smem_dst);
+  if constexpr (CG == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(d), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(d), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
 }
+template <int CG>
+__device__ __forceinline__ void dealloc_cg(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// A and B in shared memory
+template <int CG>
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  if constexpr (CG == 1)
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+                 : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+                 "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+                 : "memory");
+}
+// A in tensor memory: lane = row, one 32-bit column = two elements of K
+template <int CG>
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  if constexpr (CG == 1)
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+                 "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+                 : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+                 "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+                 : "memory");
+}
+// arrive on the mbarrier (of both blocks of a pair) when all MMAs that this thread issued so far are done
+template <int CG>
+__device__ __forceinline__ void commit_cg(uint64_t* bar) {
+  const uint32_t b = (uint32_t)__cvta_generic_to_shared(bar);
+  if constexpr (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(b),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+
 // 32 lanes x 32 columns, without the wait (wait_ld before the values are used)
 __device__ __forceinline__ void ld_32x32b_x32_async(uint32_t taddr, uint32_t* r) {
   asm volatile(
