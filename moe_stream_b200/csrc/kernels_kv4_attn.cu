@@ -20,9 +20,12 @@
 //   s = sum over the groups of (d R + o Q) + d P.
 // The first part is one more product of the stored (d, o) pairs with R and Q, each cut into two f16 (22 bits);
 // the second is one f32 multiply-add a group.  Values: v = fma(16 + c, d, o) in f16 pairs of two keys, the probabilities in f16 (bf16 would
-// cost 8 times their rounding) transposed by movmatrix from the score layout.  The running maximum is raised
+// cost 8 times their rounding; with f16 outputs, where it shows, their rests in a second product) transposed by
+// movmatrix from the score layout.  The running maximum is raised
 // only when the probabilities of a tile grow beyond 2^8: p stays far inside f16, and most tiles need no
 // reduction over the lanes.
+#include <type_traits>
+
 #include "../../include/moestream_cuda.h"
 #include "attn_types.cuh"
 #include "common.cuh"
@@ -219,7 +222,7 @@ struct Rows {
 };
 
 // one tile: scores, probabilities, value product.  MASKED: some keys are not every row's
-template <int HD, int NT, bool MASKED>
+template <int HD, int NT, bool MASKED, bool RESTS>
 __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const Bases& K, const uint8_t* tile, int key0, int len, int window,
                                           uint32_t have) {
   constexpr int G = HD / 32, TB = 256 / HD, BLK = 20 * HD, MT = HD / 16;
@@ -335,11 +338,17 @@ __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const Bases& K, const
   // transposed probabilities hold keys 2 t, 2 t + 1 (p0) and 2 t + 8, 2 t + 9 (p1) of row g (columns)
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
-    uint32_t p0[NT], p1[NT];
+    uint32_t p0[NT], p1[NT], r0[NT], r1[NT];               // r: what f16 left of p
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      p0[n] = transpose8x8(pack2<__half>(p[b][n][0], p[b][n][1]));
-      p1[n] = transpose8x8(pack2<__half>(p[b][n][2], p[b][n][3]));
+      const uint32_t x = pack2<__half>(p[b][n][0], p[b][n][1]), y = pack2<__half>(p[b][n][2], p[b][n][3]);
+      p0[n] = transpose8x8(x);
+      p1[n] = transpose8x8(y);
+      if (RESTS) {
+        const float2 fx = unpack2<__half>(x), fy = unpack2<__half>(y);
+        r0[n] = transpose8x8(pack2<__half>(p[b][n][0] - fx.x, p[b][n][1] - fx.y));
+        r1[n] = transpose8x8(pack2<__half>(p[b][n][2] - fy.x, p[b][n][3] - fy.y));
+      }
     }
     const uint8_t* blk = tile + b * BLK;
     uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;   // halves of the two pairs that are tokens of the sequence
@@ -363,6 +372,10 @@ __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const Bases& K, const
         for (int n = 0; n < NT; ++n) {
           mma_add(R.o[n][first + 2 * i], a0, a1, a2, a3, p0[n], p1[n]);
           mma_add(R.o[n][first + 2 * i + 1], a4, a5, a6, a7, p0[n], p1[n]);
+          if (RESTS) {
+            mma_add(R.o[n][first + 2 * i], a0, a1, a2, a3, r0[n], r1[n]);
+            mma_add(R.o[n][first + 2 * i + 1], a4, a5, a6, a7, r0[n], r1[n]);
+          }
         }
       }
     };
@@ -464,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     const int len = cur.s.len;
     if (threadIdx.x == 0 && begins && cur.job == 0 && a.lens[cur.seq] != len) atomicOr(err, EF_BAD_INDEX);
 
+    constexpr bool RESTS = std::is_same<T, __half>::value;
     const Bases K;
     Rows<HD, NT> R;
 #pragma unroll
@@ -540,9 +554,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
       const uint32_t have = landed ? sm.have[warp][stage] : 0u;
       const int key0 = (cur.s.first + cur.tile + x - at) * TT;
       if (key0 >= lo_all && key0 + TT - 1 <= hi_all && have == (1u << TB) - 1)
-        take_tile<HD, NT, false>(R, K, sm.stage[warp][stage], key0, len, window, have);
+        take_tile<HD, NT, false, RESTS>(R, K, sm.stage[warp][stage], key0, len, window, have);
       else
-        take_tile<HD, NT, true>(R, K, sm.stage[warp][stage], key0, len, window, have);
+        take_tile<HD, NT, true, RESTS>(R, K, sm.stage[warp][stage], key0, len, window, have);
       ++used;
       __syncwarp();                                          // the stage is free
       if (next < count) fetch_next(stage);

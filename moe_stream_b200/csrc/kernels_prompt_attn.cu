@@ -64,6 +64,8 @@ __device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x,
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // ---- pairs of f32 in one 64-bit register (one instruction for both) ----
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
   uint64_t r;
@@ -104,18 +106,17 @@ __device__ __forceinline__ Place find_place(const ms_prompt_attn& a, int n_tok, 
   Place p;
   p.ok = false;
   // blocks of all sequences; this one counts from the last, so that the longest rows of a prompt start first
-  int total = 0;
-  for (int b = 0; b < a.n_seqs; b += 32) {
-    const int i = b + lane;
-    const int n = i < a.n_seqs ? (max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) + per - 1) / per : 0;
-    total += __reduce_add_sync(0xffffffffu, n);
-  }
+  auto blocks_of = [&](int i) {
+    return i < a.n_seqs ? (max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) + per - 1) / per : 0;
+  };
+  const int n0 = blocks_of(lane);          // of the first 32, kept
+  int total = __reduce_add_sync(0xffffffffu, n0);
+  for (int b = 32; b < a.n_seqs; b += 32) total += __reduce_add_sync(0xffffffffu, blocks_of(b + lane));
   index = total - 1 - index;
   if (index < 0) return p;
   int at = 0;
   for (int b = 0; b < a.n_seqs; b += 32) {
-    const int i = b + lane;
-    const int n = i < a.n_seqs ? (max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) + per - 1) / per : 0;
+    const int n = b ? blocks_of(b + lane) : n0;
     int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -181,10 +182,8 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CL == 2 ? cluster_rank() : 0, index = blockIdx.x / CL;
   const int head = index % a.kv_heads, rep = a.heads / a.kv_heads;
-  const Place pl = find_place<HD, CL>(a, n_tok, index / a.kv_heads, err);
-  if (!pl.ok) return;                      // both blocks of a pair
-
   if (warp == S::SOFTMAX_WARPS) umma::alloc_cg<CL>(&tmem_base, S::COLS);
+  if (warp == S::SOFTMAX_WARPS + 1 && lane < 3) prefetch_map(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map);
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     mbar_init(&q_other, 1);
@@ -196,10 +195,15 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
     for (int i = 0; i < NQ; ++i) mbar_init(&o_full[i], 1);
     fence_mbar_init();
   }
+  const Place pl = find_place<HD, CL>(a, n_tok, index / a.kv_heads, err);
   umma::fence_before_sync();
   __syncthreads();
   if (CL == 2) cluster_sync();
   umma::fence_after_sync();
+  if (!pl.ok) {                            // all threads, in both blocks of a pair
+    if (warp == S::SOFTMAX_WARPS) umma::dealloc_cg<CL>(tmem_base, S::COLS);
+    return;
+  }
   constexpr uint32_t tmem = 0;             // all 512 columns are this block's, so they start at 0
   if (threadIdx.x == 0 && tmem_base != tmem) atomicOr(err, EF_BAD_SHAPE);
   const int nq = pl.q1 - pl.q0, nk = pl.k1 - pl.k0;
