@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
           f = exp2_fast(m - mm);
           den = l * f + exp2_fast(sink - mm);
         }
-        f /= den;
+        f = den > 0.f ? f / den : 0.f;       // (an infinite sink takes everything)
       }
       T* dst = (T*)a.out + (int64_t)(pl.q0 + tok) * a.out_stride + h * HD;
 #pragma unroll

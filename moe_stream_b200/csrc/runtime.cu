@@ -1714,6 +1714,7 @@ ms_status check_prompt(const ms_prompt_attn& a, const char** why) {
   if (a.n_seqs < 0 || a.total_q < 0 || a.total_k < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads)
     return *why = "counts >= 0 and heads a multiple of kv_heads required", MS_ERR_SHAPE;
   if (a.heads / a.kv_heads > 128) return *why = "at most 128 heads per kv head", MS_ERR_SHAPE;
+  if (((int64_t)a.total_q + a.n_seqs) * a.kv_heads > 0x3fffffffll) return *why = "too many rows", MS_ERR_SHAPE;
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return *why = "head_dim 64, 128 or 256 required", MS_ERR_SHAPE;
   if (!elem_type(a.type, false)) return *why = "f16 or bf16 required", MS_ERR_UNSUPPORTED_QTYPE;
   const int64_t q = (int64_t)a.heads * a.head_dim, k = (int64_t)a.kv_heads * a.head_dim;
@@ -1732,8 +1733,8 @@ ms_status check_prompt(const ms_prompt_attn& a, const char** why) {
 }
 
 ms_status check_cache(const ms_kv4_cache& c, const char** why) {
-  if (c.kv_heads <= 0 || c.n_pages < 0 || c.n_seqs < 0 || c.max_pages < 0)
-    return *why = "kv_heads > 0 and counts >= 0 required", MS_ERR_SHAPE;
+  if (c.kv_heads <= 0 || c.kv_heads > 65536 || c.n_pages < 0 || c.n_seqs < 0 || c.max_pages < 0)
+    return *why = "kv_heads in 1 .. 65536 and counts >= 0 required", MS_ERR_SHAPE;
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return *why = "head_dim 64, 128 or 256 required", MS_ERR_SHAPE;
   if (c.page_tokens < 16 || c.page_tokens > 1024 || (c.page_tokens & (c.page_tokens - 1)))
     return *why = "page_tokens must be a power of two in 16 .. 1024", MS_ERR_SHAPE;
@@ -1803,6 +1804,7 @@ ms_status ms_prompt_attention(ms_ctx* c, const ms_prompt_attn* args) {
   if (st != MS_OK) return fail(c, st, "prompt_attention: %s", why);
   if (!c) return MS_ERR_INVALID_ARG;
   if (a.scale == 0.0f) a.scale = (float)(1.0 / std::sqrt((double)a.head_dim));
+  if (a.window >= a.total_k) a.window = 0;   // hides no key
   OnDevice on(c->device);
   MS_CUDA(c, launch_prompt_attention(c->dc, a, c->stream));
   return MS_OK;
@@ -1853,6 +1855,7 @@ ms_status ms_kv4_attention(ms_ctx* c, const ms_kv4_cache* kv, const ms_kv4_attn*
   if (a.work_bytes < kv4_attn_workspace(c->dc, *kv, a.n_query, a.heads))
     return fail(c, MS_ERR_SHAPE, "kv4_attention: the workspace is smaller than ms_kv4_attention_workspace says");
   if (a.scale == 0.0f) a.scale = (float)(1.0 / std::sqrt((double)kv->head_dim));
+  if (a.window >= kv->max_pages * kv->page_tokens) a.window = 0;   // hides no key
   OnDevice on(c->device);
   MS_CUDA(c, launch_kv4_attention(c->dc, *kv, a, c->stream));
   return MS_OK;

@@ -57,13 +57,13 @@ def test_rope_refusals(L, change, status):
     (dict(heads=258, q_stride=1 << 15, out_stride=1 << 15), SHAPE), (dict(head_dim=96, q_stride=4096), SHAPE),
     (dict(type=0), QTYPE), (dict(type=8), QTYPE), (dict(q_stride=504), SHAPE), (dict(v_stride=132), SHAPE),
     (dict(k=P + 8), SHAPE), (dict(out=P + 2), SHAPE), (dict(scale=-1.0), INVALID), (dict(scale=float("inf")), INVALID),
-    (dict(cu_q=None), INVALID), (dict(v=None), INVALID), (dict(out=P), INVALID),
+    (dict(cu_q=None), INVALID), (dict(v=None), INVALID), (dict(out=P), INVALID), (dict(total_q=1 << 30), SHAPE),
 ], ids=str)
 def test_prompt_refusals(L, change, status):
     assert L.ms_prompt_attention(None, C.byref(make(_lib.PromptAttn, **{**PROMPT, **change}))) == status
 
 
-CACHE_BAD = [(dict(kv_heads=0), SHAPE), (dict(head_dim=96), SHAPE), (dict(page_tokens=8), SHAPE), (dict(page_tokens=48), SHAPE),
+CACHE_BAD = [(dict(kv_heads=0), SHAPE), (dict(kv_heads=70000), SHAPE), (dict(head_dim=96), SHAPE), (dict(page_tokens=8), SHAPE), (dict(page_tokens=48), SHAPE),
              (dict(page_tokens=2048), SHAPE), (dict(pages=P + 4), SHAPE), (dict(pages=None), INVALID),
              (dict(block_table=None), INVALID), (dict(max_pages=1 << 28), SHAPE), (dict(n_seqs=-1), SHAPE)]
 
@@ -83,7 +83,7 @@ def test_cache_row_refusals(L, cache, rows, status):
 @pytest.mark.parametrize("cache,attn,status", [
     ({}, {}, INVALID), *[(c, {}, s) for c, s in CACHE_BAD],
     ({}, dict(n_query=0), SHAPE), ({}, dict(heads=9), SHAPE), ({}, dict(n_query=33), SHAPE), ({}, dict(type=0), QTYPE),
-    (dict(n_seqs=70000), {}, SHAPE),
+    (dict(n_seqs=70000), {}, SHAPE), (dict(n_seqs=60000, max_pages=1 << 20), {}, SHAPE),
     ({}, dict(scale=float("nan")), INVALID), ({}, dict(q=P + 2), SHAPE), ({}, dict(work=P + 8), SHAPE),
     ({}, dict(lens=None), INVALID), ({}, dict(work=None), INVALID), ({}, dict(out=P), INVALID),
 ], ids=str)

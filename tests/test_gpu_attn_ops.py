@@ -477,6 +477,135 @@ def test_prompt_attention_bad_offsets_are_reported(ctx):
     assert (out[20:] == 7.0).all() and (out[:20] != 7.0).any()
 
 
+# ---------------------------------------------------------------- far offsets, wide windows, infinite sinks, two streams
+
+def far_rows(rows, heads, hd, t, stride=1 << 22):
+    """[rows, heads, hd] whose last rows lie beyond 2^32 bytes: a view with a wide stride."""
+    base = torch.empty((rows - 1) * stride + heads * hd, dtype=t, device="cuda")
+    return base.as_strided((rows, heads, hd), (stride, hd, 1))
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """1030 rows 2^22 elements apart span 8.6 GB; the cache's pool has 5 GB of pages, the last ones in use."""
+    from moe_stream_b200.engine import KV4Cache
+    n, H, kv, hd, t = 1030, 4, 2, 64, torch.bfloat16
+    g = gen(1)
+    near = lambda heads: torch.randn(n, heads, hd, device="cuda", generator=g).to(t)
+    q, k, v = near(H), near(kv), near(kv)
+    cos, sin = torch.ones(n, 32, device="cuda"), torch.zeros(n, 32, device="cuda")
+    far = far_rows(n, H, hd, t)
+    far.copy_(q)
+    ko = torch.empty_like(k)
+    ctx.qk_norm_rope(far, k, None, None, 0.0, cos, sin, torch.arange(n, device="cuda", dtype=torch.int32), far, ko)
+    ctx.sync()
+    assert torch.equal(far, q) and torch.equal(ko, k)
+    cu, out = i32([0, n]), torch.empty_like(q)
+    ctx.prompt_attention(q, k, v, cu, cu, out)
+    ctx.prompt_attention(far, k, v, cu, cu, far_out := far_rows(n, H, hd, t))
+    ctx.sync()
+    assert torch.equal(out, far_out)
+    del far_out
+    fk = far_rows(n, kv, hd, t)
+    fk.copy_(k)
+    again = torch.empty_like(out)
+    ctx.prompt_attention(q, fk, v, cu, cu, again)
+    ctx.sync()
+    assert torch.equal(out, again)
+    per = KV4Cache.page_bytes(kv, hd, 16)
+    pool = (5 << 30) // per
+    pages = torch.empty(pool * per, dtype=torch.uint8, device="cuda")
+    need = -(-n // 16)
+    table = torch.arange(pool - need, pool, dtype=torch.int32, device="cuda")[None]
+    cache = KV4Cache(pages, table, kv, hd, 16)
+    ctx.kv4_write(cache, fk, v, cu, i32([0]))
+    small = KV4Cache(pages[(pool - need) * per:].clone(), torch.arange(need, dtype=torch.int32, device="cuda")[None], kv, hd, 16)
+    o = [torch.empty(1, 1, H, hd, dtype=t, device="cuda") for _ in range(2)]
+    for c, x in zip((cache, small), o):
+        work = torch.empty(ctx.kv4_attention_workspace_bytes(c, 1, 1, H), dtype=torch.uint8, device="cuda")
+        ctx.kv4_attention(c, q[:1, None].contiguous(), i32([n]), x, work)
+        ctx.sync()
+    assert torch.equal(*o)
+    back = [torch.empty(n, kv, hd, dtype=t, device="cuda") for _ in range(2)]
+    ctx.kv4_read(cache, cu, i32([0]), fk, back[1])
+    ctx.kv4_read(small, cu, i32([0]), back[0], back[1])
+    ctx.sync()
+    assert torch.equal(fk, back[0])
+
+
+def test_windows_wider_than_anything(ctx):
+    """The largest window is no window."""
+    case = ([100, 30], 2, 16, 8, 1, 64, 0, False, "bfloat16")
+    cache, table, q, lens, out, work, _, _ = cached_case(ctx, case, poison=True)
+    ctx.kv4_attention(cache, q, lens, out, work)
+    wide = torch.empty_like(out)
+    ctx.kv4_attention(cache, q, lens, wide, work, window=2 ** 31 - 1)
+    pq, pk, pv, cq, ck, _, _ = prompt_case([70, 40], [0, 9], 8, 2, 64, torch.bfloat16)
+    po = [torch.empty_like(pq) for _ in range(2)]
+    ctx.prompt_attention(pq, pk, pv, cq, ck, po[0])
+    ctx.prompt_attention(pq, pk, pv, cq, ck, po[1], window=2 ** 31 - 1)
+    ctx.sync()
+    assert torch.equal(out, wide) and torch.equal(po[0][:110], po[1][:110])
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_infinite_sinks(ctx, hd):
+    """A sink of -infinity is none, one of +infinity takes everything."""
+    H = 8
+    case = ([300, 0, 41], 1, 16, H, 2, hd, 0, False, "float16")
+    cache, table, q, lens, out, work, _, _ = cached_case(ctx, case, poison=True)
+    pq, pk, pv, cq, ck, _, _ = prompt_case([70, 40], [0, 9], H, 2, hd, torch.float16)
+    sk = torch.full((H,), float("-inf"), device="cuda")
+    sk[3] = float("inf")
+    so, ps, po = torch.empty_like(out), torch.empty_like(pq), torch.empty_like(pq)
+    ctx.kv4_attention(cache, q, lens, out, work)
+    ctx.kv4_attention(cache, q, lens, so, work, sinks=sk)
+    ctx.prompt_attention(pq, pk, pv, cq, ck, po)
+    ctx.prompt_attention(pq, pk, pv, cq, ck, ps, sinks=sk)
+    ctx.sync()
+    keep = [h for h in range(H) if h != 3]
+    assert (so[:, :, 3] == 0).all() and torch.equal(so[:, :, keep], out[:, :, keep])
+    assert (ps[:110, 3] == 0).all() and torch.equal(ps[:110, keep], po[:110, keep])
+
+
+def test_two_streams_at_once(ctx):
+    """Both attentions running on two streams, each call with its own workspace and outputs."""
+    from moe_stream_b200.engine import Context
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    cs = [Context(0, stream=s) for s in streams]
+    sets = []
+    for i, hd in enumerate((64, 128, 256)):
+        case = ([3000, 200, 17], 1, 32, 16, 2, hd, 0, False, "bfloat16")
+        kv = cached_case(ctx, case, poison=True, seed=i)
+        pr = prompt_case([300, 90], [100, 0], 16, 2, hd, torch.bfloat16, seed=i)
+        want = torch.empty_like(kv[4]), torch.empty_like(pr[0])
+        ctx.kv4_attention(kv[0], kv[2], kv[3], want[0], kv[5])
+        ctx.prompt_attention(*pr[:5], want[1])
+        sets.append((kv, pr, want))
+    ctx.sync()
+    torch.cuda.synchronize()
+    outs = []
+    for r in range(10):
+        for c in cs:
+            for kv, pr, want in sets:
+                o = torch.full_like(kv[4], 7.0), torch.full_like(pr[0], 7.0), torch.empty_like(kv[5])
+                outs.append((o, want))
+    torch.cuda.synchronize()
+    k = 0
+    for r in range(10):
+        for c in cs:
+            for kv, pr, want in sets:
+                o = outs[k][0]
+                k += 1
+                c.kv4_attention(kv[0], kv[2], kv[3], o[0], o[2])
+                c.prompt_attention(*pr[:5], o[1])
+    for c in cs:
+        c.sync()
+    for o, want in outs:
+        assert torch.equal(o[0], want[0]) and torch.equal(o[1][:390], want[1][:390])
+    for c in cs:
+        c.close()
+
+
 # ---------------------------------------------------------------- together
 
 def test_chain_prompt_then_decode(ctx):
