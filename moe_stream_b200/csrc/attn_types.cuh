@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace ms {
@@ -95,6 +96,24 @@ __device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seqs, int j) 
     else hi = mid - 1;
   }
   return lo;
+}
+
+// Launch a kernel; a small grid may start while its predecessor in the stream ends (the kernel calls pdl_wait_prior
+// before it touches memory), which saves a decode step about a microsecond a kernel.  The waiting blocks of a large
+// grid would only take room from the predecessor: a cache write and read of 8,900 tokens took 21.7 us so, 19.1 without.
+// The error is left to cudaGetLastError.
+template <class... P, class... A>
+inline void launch_early(void (*kernel)(P...), uint32_t grid, uint32_t threads, cudaStream_t s, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = grid <= 296 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 }  // namespace ms

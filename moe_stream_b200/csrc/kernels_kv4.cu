@@ -27,6 +27,8 @@ struct Leads {
   int n;
 };
 __device__ __forceinline__ void find_leads(const ms_kv4_cache& c, const ms_kv4_rows& r, int rows, Leads& ls, uint32_t* err) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, j = blockIdx.x * rows + lane;
     bool lead = false;
@@ -286,8 +288,8 @@ cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_rows& r, 
   int rows = kRows;
   while (rows > 2 && (int64_t)r.total < (int64_t)rows * 4 * d.sm_count) rows /= 2;
   const uint32_t grid = (uint32_t)(((int64_t)r.total + rows - 1) / rows);
-  if (write) kv4_write_kernel<T, HD><<<grid, kThreads, 0, s>>>(c, r, rows, d.err);
-  else kv4_read_kernel<T, HD><<<grid, kThreads, 0, s>>>(c, r, rows, d.err);
+  if (write) launch_early(kv4_write_kernel<T, HD>, grid, kThreads, s, c, r, rows, d.err);
+  else launch_early(kv4_read_kernel<T, HD>, grid, kThreads, s, c, r, rows, d.err);
   return cudaGetLastError();
 }
 

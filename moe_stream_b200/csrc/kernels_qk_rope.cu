@@ -16,31 +16,30 @@ namespace {
 
 constexpr int kThreads = 128;
 
-// One group of LPR = head_dim / 16 lanes holds a head: two chunks of 8 dims per lane, the two sides of its
-// rotation pairs where it rotates (dims 8 l .. and rot / 2 + 8 l ..), otherwise dims 16 l .. 16 l + 15.  A group
-// takes HPG heads of one token, whose table row and norm weights stay in registers.
+// One group of LPR = head_dim / 16 lanes holds a head: two chunks of 8 dims per lane.  The first rot / 16 lanes hold
+// the dims that rotate, 8 l .. and rot / 2 + 8 l .. (the two sides of their pairs, or 4 pairs of neighbours in each),
+// the others share the rest the same way, so that the lanes of a load read neighbouring chunks.  A group takes
+// HPG heads of one token, whose table row and norm weights stay in registers.
 template <class TI, class TO, int LPR, int HPG, bool INTER>
-__global__ void __launch_bounds__(kThreads) qk_rope_kernel(const ms_qk_rope a, uint32_t* err) {
+__global__ void __launch_bounds__(kThreads, 5) qk_rope_kernel(const ms_qk_rope a, uint32_t* err) {
   const int lane = threadIdx.x % LPR;
   const uint32_t item = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
   const uint32_t nbq = (a.heads + HPG - 1) / HPG, nb = nbq + (a.kv_heads + HPG - 1) / HPG;
   const uint32_t t = item / nb, hb = item % nb;
   const bool is_q = hb < nbq;
   const int h0 = (is_q ? hb : hb - nbq) * HPG, nh = is_q ? a.heads : a.kv_heads;
-  bool live = t < (uint32_t)a.n_tokens;
-  int pos = 0;
-  if (live) {
-    pos = a.pos[t];
-    if (pos < 0 || pos >= a.max_pos) {
-      if (hb == 0 && lane == 0) atomicOr(err, EF_BAD_INDEX);
-      live = false;
-    }
-  }
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const bool in = t < (uint32_t)a.n_tokens;
+  const int pos = in ? a.pos[t] : 0;
+  // (loads that did not wait for the position took 65 us for 57 on a prompt of 16,384 tokens)
+  const bool live = in && pos >= 0 && pos < a.max_pos;
+  if (in && !live && hb == 0 && lane == 0) atomicOr(err, EF_BAD_INDEX);
   constexpr int HD = LPR * 16;
   const unsigned mask = (LPR == 32 ? 0xffffffffu : (1u << LPR) - 1) << (threadIdx.x % 32 / LPR * LPR);   // the lanes of the head
-  const int half = a.rot_dim / 2;
-  const bool turns = 16 * lane < a.rot_dim;
-  const int d0 = !INTER && turns ? 8 * lane : 16 * lane, d1 = !INTER && turns ? d0 + half : d0 + 8;
+  const int half = a.rot_dim / 2, nt = a.rot_dim / 16;
+  const bool turns = lane < nt;
+  const int d0 = turns ? 8 * lane : a.rot_dim + 8 * (lane - nt), d1 = d0 + (turns ? half : 8 * (LPR - nt));
   const TI* src = (const TI*)(is_q ? a.q : a.k) + (int64_t)t * (is_q ? a.q_stride : a.k_stride);
   TO* dst = (TO*)(is_q ? a.q_out : a.k_out) + (int64_t)t * (is_q ? a.q_out_stride : a.k_out_stride);
   Raw8<TI> r[HPG][2];
@@ -50,13 +49,13 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const ms_qk_rope a, u
       r[i][0].load(src + (h0 + i) * HD + d0);
       r[i][1].load(src + (h0 + i) * HD + d1);
     }
-  // 8 pairs per lane, (8 l + i, half + 8 l + i) or 2 i and 2 i + 1 of its 16 dims, and the 16 weights
+  // the angles of its 8 pairs (d0 + i, d1 + i), or of 4 neighbours' pairs in each chunk, and its 16 weights
   float4 cs[2], sn[2], w[4];
   if (live && turns) {
-    const float4* c4 = reinterpret_cast<const float4*>(a.cos_t + (int64_t)pos * half + 8 * lane);
-    const float4* s4 = reinterpret_cast<const float4*>(a.sin_t + (int64_t)pos * half + 8 * lane);
-    cs[0] = c4[0]; cs[1] = c4[1];
-    sn[0] = s4[0]; sn[1] = s4[1];
+    const int i0 = INTER ? d0 / 2 : d0, i1 = INTER ? d1 / 2 : d0 + 4;
+    const float *ct = a.cos_t + (int64_t)pos * half, *st = a.sin_t + (int64_t)pos * half;
+    cs[0] = *reinterpret_cast<const float4*>(ct + i0); cs[1] = *reinterpret_cast<const float4*>(ct + i1);
+    sn[0] = *reinterpret_cast<const float4*>(st + i0); sn[1] = *reinterpret_cast<const float4*>(st + i1);
   }
   const float* nw = is_q ? a.q_norm : a.k_norm;
   if (nw) {
@@ -116,6 +115,8 @@ __global__ void __launch_bounds__(kThreads) qk_rope_any_kernel(const ms_qk_rope 
   const uint32_t item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), nh = a.heads + a.kv_heads;
   const uint32_t t = item / nh;
   const int hh = item % nh;
+  pdl_wait_prior();
+  pdl_launch_dependents();
   if (t >= (uint32_t)a.n_tokens) return;
   const int pos = a.pos[t];
   if (pos < 0 || pos >= a.max_pos) {
@@ -155,8 +156,8 @@ template <class TI, class TO, int LPR, int HPG>
 void start_vec(const ms_qk_rope& a, uint32_t* err, cudaStream_t s) {
   const uint32_t nb = (a.heads + HPG - 1) / HPG + (a.kv_heads + HPG - 1) / HPG;
   const uint32_t grid = ((uint64_t)a.n_tokens * nb + kThreads / LPR - 1) / (kThreads / LPR);
-  if (a.interleaved) qk_rope_kernel<TI, TO, LPR, HPG, true><<<grid, kThreads, 0, s>>>(a, err);
-  else qk_rope_kernel<TI, TO, LPR, HPG, false><<<grid, kThreads, 0, s>>>(a, err);
+  if (a.interleaved) launch_early(qk_rope_kernel<TI, TO, LPR, HPG, true>, grid, kThreads, s, a, err);
+  else launch_early(qk_rope_kernel<TI, TO, LPR, HPG, false>, grid, kThreads, s, a, err);
 }
 
 template <class TI, class TO>
@@ -168,7 +169,7 @@ void start(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
                    aligned16(a.q_norm) && aligned16(a.k_norm);
   if (!vec) {
     const uint64_t items = (uint64_t)a.n_tokens * (a.heads + a.kv_heads);
-    qk_rope_any_kernel<TI, TO><<<(uint32_t)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, s>>>(a, c.err);
+    launch_early(qk_rope_any_kernel<TI, TO>, (uint32_t)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, s, a, c.err);
     return;
   }
   // few rows: one head per group, so that the loads of a decode step spread over the SMs
