@@ -24,6 +24,12 @@
 // movmatrix from the score layout.  The running maximum is raised
 // only when the probabilities of a tile grow beyond 2^8: p stays far inside f16, and most tiles need no
 // reduction over the lanes.
+//
+// Measured: 32 sequences of 8,300 tokens on average, 4 heads of 128 dims (162 MB): 43 us, 3.7 TB/s; one of 131,072
+// tokens, 8 heads of 64 dims (84 MB, f16): 29 us; one of 4,097 tokens: 9 us.  Bulk copies alone stream the first
+// in 30 us; 3 us go by before the first copy (lengths, split, page numbers), the blocks end up to 4 us apart, and the
+// second kernel takes 3 to 4 us.  The loop issues 330 instructions a warp for 16 tokens of 128 dims and keeps the
+// issue slots half busy.
 #include <type_traits>
 
 #include "../../include/moestream_cuda.h"

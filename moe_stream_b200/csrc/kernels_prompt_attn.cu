@@ -7,17 +7,29 @@
 // once for the group and short sequences still fill a tile.  A block holds NQ query tiles of one sequence (2; 1
 // with 256 dims, whose output takes half of the tensor memory) and walks over the keys in tiles of BN.
 //
-// Warps: NQ groups of 4 for the softmax, one that issues the MMAs, one that issues the TMA copies.  Steps
+// Warps: NQ groups of 4 for the softmax, one that issues the MMAs, two that issue the TMA copies (K and V).  Steps
 // s = 0, 1, ... alternate between two score buffers in tensor memory: with NQ = 2 step s is query tile s & 1 and
 // key tile s / 2, with NQ = 1 it is key tile s.  The MMA warp issues scores(s + 2) right after values(s), so the
 // tensor core works on one buffer while the softmax works on the other.  A softmax thread owns a row: it reads
-// the scores, writes the probabilities over them as 16-bit pairs, and the value product takes them from tensor
-// memory.  The running maximum is that of the row's first tile until the probabilities of a later one add up to more
-// than kRaise: only then the tile's maximum is looked for and the output rescaled, and no probability comes
-// near the largest f16.  Sums are in f32 over the unrounded probabilities.
+// the scores, writes the probabilities as 16-bit pairs, and the value product takes them from tensor memory.  With
+// 128 and 256 dims they lie over the scores they came from, which the MMA warp overwrites next: the MMAs of
+// one thread execute in the order of issue.  The running maximum is that of the row's first tile until the
+// probabilities of a later one add up to more than kRaise: only then the tile's maximum is looked for and the output
+// rescaled, and no probability comes near the largest f16.  Sums are in f32 over the unrounded probabilities.
 //
 // Values of keys behind the sequence's end (other rows of the packed buffer, perhaps not finite) are zeroed in
 // shared memory before the last product; their scores are masked.
+//
+// CL = 2 (256 dims): two blocks of a cluster share each MMA (M = 256), each with its own 128 rows and half of every K
+// and V tile.  With one query tile a block, 256 dims read K and V from L2 for 128 rows only, 28 bytes a cycle and
+// SM, and waited for them: a chunk of 2,048 queries behind 9,001 keys took 352 us, with pairs 238 us (337 GFLOP,
+// 1,414 TFLOP/s, 84 % of the cuBLAS rate measured on this GPU).  128 dims have two query tiles a block and lose by
+// pairs, whose two blocks wait for each other: 463 us became 526 us for 8,192 tokens of 32 heads (550 GFLOP; 463 us
+// are 1,187 TFLOP/s, 71 %).  There a key tile takes 3,900 cycles: the chain of scores (512), softmax (1,890, of which
+// 1,024 are the special-function unit's for 128 exponentials a thread), values (512) and four hand-overs of a
+// slot, two slots in turn.  What did not help there: a quarter of the exponentials as polynomials, probabilities
+// handed over in halves, an MMA warp for each slot (interleaving their MMAs costs 40 %), blocks of half the
+// tensor memory, two to an SM (64 dims: 235 us became 285, an MMA of 64 columns takes as long as one of 128).
 #include <cuda.h>
 
 #include <type_traits>
