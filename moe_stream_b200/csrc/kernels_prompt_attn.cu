@@ -194,7 +194,6 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CL == 2 ? cluster_rank() : 0, index = blockIdx.x / CL;
   const int head = index % a.kv_heads, rep = a.heads / a.kv_heads;
-  if (warp == S::SOFTMAX_WARPS) umma::alloc_cg<CL>(&tmem_base, S::COLS);
   if (warp == S::SOFTMAX_WARPS + 1 && lane < 3) prefetch_map(lane == 0 ? &q_map : lane == 1 ? &k_map : &v_map);
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
@@ -207,6 +206,9 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
     for (int i = 0; i < NQ; ++i) mbar_init(&o_full[i], 1);
     fence_mbar_init();
   }
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  if (warp == S::SOFTMAX_WARPS) umma::alloc_cg<CL>(&tmem_base, S::COLS);   // after the wait: the predecessor may hold it
   const Place pl = find_place<HD, CL>(a, n_tok, index / a.kv_heads, err);
   umma::fence_before_sync();
   __syncthreads();
@@ -553,11 +555,16 @@ cudaError_t start(const DevCtx& d, const ms_prompt_attn& a, cudaStream_t s) {
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CL;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  if (CL == 2) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CL;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  } else {                                 // may start while its predecessor in the stream ends
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = CL == 2 ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, prompt_attn_kernel<T, HD, CL>, a, q, k, v, n_tok, d.err);
 }
 
