@@ -117,32 +117,62 @@ __device__ __forceinline__ Place find_place(const ms_prompt_attn& a, int n_tok, 
   const int lane = threadIdx.x & 31, per = CL * S::NQ * n_tok;
   Place p;
   p.ok = false;
-  // blocks of all sequences; this one counts from the last, so that the longest rows of a prompt start first
+  // Blocks of all sequences, those with the most keys first, so that the last ones to start are short.  Up to 32
+  // sequences (a lane for each) are put in that order: more(c) is how many blocks of the lane's sequence have more
+  // than c key tiles in front of their last query, and the place is found by bisection over c.  More sequences are
+  // taken from the last one's last block on.
+  int nqs = 0, nks = 0;
   auto blocks_of = [&](int i) {
-    return i < a.n_seqs ? (max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) + per - 1) / per : 0;
+    nqs = i < a.n_seqs ? max(0, min(a.cu_q[i + 1], a.total_q) - max(0, a.cu_q[i])) : 0;
+    return (nqs + per - 1) / per;
   };
   const int n0 = blocks_of(lane);          // of the first 32, kept
   int total = __reduce_add_sync(0xffffffffu, n0);
   for (int b = 32; b < a.n_seqs; b += 32) total += __reduce_add_sync(0xffffffffu, blocks_of(b + lane));
-  index = total - 1 - index;
-  if (index < 0) return p;
-  int at = 0;
-  for (int b = 0; b < a.n_seqs; b += 32) {
-    const int n = b ? blocks_of(b + lane) : n0;
+  if (index >= total) return p;
+  // number `index` of the lanes' n candidates: its lane, and k, the how manieth of that lane's (-1: it is behind them)
+  int k = 0;
+  auto pick = [&](int n) {
     int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, index < at + inc);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      p.seq = b + l;
-      p.t0 = (index - at - __shfl_sync(0xffffffffu, inc - n, l)) * per;
-      break;
+    const unsigned hit = __ballot_sync(0xffffffffu, index < inc);
+    const int l = hit ? __ffs(hit) - 1 : 31;
+    k = index - __shfl_sync(0xffffffffu, hit ? inc - n : inc, l);
+    return hit ? l : -1;
+  };
+  if (a.n_seqs > 1 && a.n_seqs <= 32) {
+    nks = lane < a.n_seqs ? max(0, min(a.cu_k[lane + 1], a.total_k) - max(0, a.cu_k[lane])) : 0;
+    auto more = [&](int c) {               // blocks whose last query stands at key c BN or later
+      const int need = c * S::BN - (nks - nqs) + 1;          // tokens up to and with that query
+      return c < 0 || need <= 0 ? n0 : need > nqs ? 0 : n0 - (need - 1) / per;
+    };
+    int lo = 0, hi = __reduce_max_sync(0xffffffffu, nks) / S::BN + 1;   // the least c with more(c) <= index in all
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if ((int)__reduce_add_sync(0xffffffffu, more(mid)) <= index) hi = mid;
+      else lo = mid + 1;
     }
-    at += __shfl_sync(0xffffffffu, inc, 31);
+    const int above = more(lo);
+    index -= __reduce_add_sync(0xffffffffu, above);
+    p.seq = pick(more(lo - 1) - above);
+    p.t0 = (__shfl_sync(0xffffffffu, n0 - above - 1, p.seq) - k) * per;
+  } else {
+    index = total - 1 - index;
+    p.seq = -1;
+    for (int b = 0; b < a.n_seqs; b += 32) {
+      const int l = pick(b ? blocks_of(b + lane) : n0);
+      if (l >= 0) {
+        p.seq = b + l;
+        p.t0 = k * per;
+        break;
+      }
+      index = k;
+    }
+    if (p.seq < 0) return p;
   }
   p.q0 = a.cu_q[p.seq]; p.q1 = a.cu_q[p.seq + 1];
   p.k0 = a.cu_k[p.seq]; p.k1 = a.cu_k[p.seq + 1];
