@@ -24,12 +24,12 @@
 // and V tile.  With one query tile a block, 256 dims read K and V from L2 for 128 rows only, 28 bytes a cycle and
 // SM, and waited for them: a chunk of 2,048 queries behind 9,001 keys took 352 us, with pairs 238 us (337 GFLOP,
 // 1,414 TFLOP/s, 84 % of the cuBLAS rate measured on this GPU).  128 dims have two query tiles a block and lose by
-// pairs, whose two blocks wait for each other: 463 us became 526 us for 8,192 tokens of 32 heads (550 GFLOP; 463 us
-// are 1,187 TFLOP/s, 71 %).  There a key tile takes 3,900 cycles: the chain of scores (512), softmax (1,890, of which
+// pairs, whose two blocks wait for each other: 463 us became 526 us for 8,192 tokens of 32 heads (550 GFLOP; now
+// 459 us, 1,198 TFLOP/s, 72 %).  There a key tile takes 3,900 cycles: the chain of scores (512), softmax (1,890, of which
 // 1,024 are the special-function unit's for 128 exponentials a thread), values (512) and four hand-overs of a
 // slot, two slots in turn.  What did not help there: a quarter of the exponentials as polynomials, probabilities
-// handed over in halves, an MMA warp for each slot (interleaving their MMAs costs 40 %), blocks of half the
-// tensor memory, two to an SM (64 dims: 235 us became 285, an MMA of 64 columns takes as long as one of 128).
+// handed over in halves, two threads a row (515 us), an MMA warp for each slot (interleaving their MMAs costs 40 %),
+// blocks of half the tensor memory, two to an SM (64 dims: 235 us became 285, an MMA of 64 columns takes as long as one of 128).
 #include <cuda.h>
 
 #include <type_traits>
@@ -326,71 +326,95 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
       // descriptors of the first tiles; others are that many 16-byte units further
       const uint64_t dq = umma::smem_desc_sw128(sq, 0), dk = umma::smem_desc_sw128(sk, 0), dv = umma::smem_desc_sw128(sv, BN * 128);
       const bool one = umma::elect();
-      auto free_stage = [&](uint64_t* bar, int j) {          // only where a copy waits for it: none is left open at the end
-        if (one && j + ST < pl.tiles) umma::commit_cg<CL>(bar);
-        __syncwarp();
+      // A step is the value product of a query tile and the scores after it.  slot is a constant: its addresses are, too.
+      bool alive = pl.tiles > 0;
+      auto need = [&](uint64_t* bar, uint64_t* bar_other, int parity) {
+        alive = alive && wait(bar, parity) && (CL == 1 || bar_other == nullptr || wait(bar_other, parity));
       };
-      bool alive = pl.tiles > 0 && wait(&q_full, 0) && (CL == 1 || wait(&q_other, 0));
-      // slot is a constant: its addresses are, too (a block issues an MMA every 64 cycles)
-      auto scores = [&](auto slot_c, int j) {
-        constexpr int slot = decltype(slot_c)::value;
-        if (!alive || j >= pl.tiles) return;
-        const int st = j % ST;
-        if (NQ == 1 || slot == 0) {
-          alive = wait(&k_full[st], j / ST) && (CL == 1 || wait(&k_other[st], j / ST));
-          if (!alive) return;
-          umma::fence_after_sync();
-        }
-        if (NQ == 1 || slot < slots) {
-          if (one) {
-            const uint64_t q = dq + (NQ == 2 ? slot : 0) * (S::Q_BYTES >> 4), k = dk + st * (S::KV_BYTES >> 4);
-#pragma unroll
-            for (int b = 0; b < BLK; ++b)
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                umma::mma_ss<CL>(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, k + (b * S::K_ROWS * 128 + kk * 32) / 16, id_s, b || kk);
-            umma::commit_cg<CL>(&s_full[slot]);
-          }
-          __syncwarp();
-        }
-        if (NQ == 1 || slot == 1) free_stage(&k_empty[st], j);
+      auto need_k = [&](int j) {
+        if (j < pl.tiles) need(&k_full[j % ST], &k_other[j % ST], j / ST);
       };
-      auto values = [&](auto slot_c, int j) {
+      auto need_v = [&](int j) {
+        need(&v_full[j % ST], &v_other[j % ST], j / ST);
+        if (alive && clear_tail(j) && CL == 2) fence_cluster();
+      };
+      auto scores = [&](auto slot_c, int j) {                // one thread; K of tile j has arrived
         constexpr int slot = decltype(slot_c)::value;
-        if (!alive || j >= pl.tiles) return;
         const int st = j % ST;
-        if (NQ == 1 || slot == 0) {
-          alive = wait(&v_full[st], j / ST) && (CL == 1 || wait(&v_other[st], j / ST));
-          if (!alive) return;
-          if (clear_tail(j) && CL == 2) fence_cluster();
-        }
         if (NQ == 1 || slot < slots) {
-          const int turn = NQ == 2 ? j : j >> 1;               // how often this buffer was filled before
-          alive = wait(&p_full[slot], turn);
-          if (!alive) return;
-          umma::fence_after_sync();
-          if (one) {
-            const uint64_t v = dv + st * (S::KV_BYTES >> 4);
+          const uint64_t q = dq + (NQ == 2 ? slot : 0) * (S::Q_BYTES >> 4), k = dk + st * (S::KV_BYTES >> 4);
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              umma::mma_ts<CL>(S::O_COL + (NQ == 2 ? slot * HD : 0), S::P_COL + slot * S::P_STEP + kk * 8, v + kk * 2048 / 16, id_o,
-                               j > 0 || kk > 0);
-            umma::commit_cg<CL>(&o_full[NQ == 2 ? slot : 0]);
-          }
-          __syncwarp();
+          for (int b = 0; b < BLK; ++b)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma::mma_ss<CL>(slot * BN, q + (b * 128 * 128 + kk * 32) / 16, k + (b * S::K_ROWS * 128 + kk * 32) / 16, id_s, b || kk);
+          umma::commit_cg<CL>(&s_full[slot]);
         }
-        if (NQ == 1 || slot == 1) free_stage(&v_empty[st], j);
+        // (a place is released only where a copy waits for it: no arrival is left open at the end)
+        if ((NQ == 1 || slot == 1) && j + ST < pl.tiles) umma::commit_cg<CL>(&k_empty[st]);
+      };
+      auto values = [&](auto slot_c, int j) {                // one thread; V of tile j and the slot's probabilities are there
+        constexpr int slot = decltype(slot_c)::value;
+        const int st = j % ST;
+        if (NQ == 1 || slot < slots) {
+          const uint64_t v = dv + st * (S::KV_BYTES >> 4);
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            umma::mma_ts<CL>(S::O_COL + (NQ == 2 ? slot * HD : 0), S::P_COL + slot * S::P_STEP + kk * 8, v + kk * 2048 / 16, id_o,
+                             j > 0 || kk > 0);
+          umma::commit_cg<CL>(&o_full[NQ == 2 ? slot : 0]);
+        }
+        if ((NQ == 1 || slot == 1) && j + ST < pl.tiles) umma::commit_cg<CL>(&v_empty[st]);
       };
       constexpr std::integral_constant<int, 0> s0;
       constexpr std::integral_constant<int, 1> s1;
-      scores(s0, 0);
-      scores(s1, NQ == 2 ? 0 : 1);
-      for (int j = 0; j < pl.tiles && alive; j += NQ == 2 ? 1 : 2) {
-        const int j1 = NQ == 2 ? j : j + 1, ahead = NQ == 2 ? 1 : 2;
-        values(s0, j);
-        scores(s0, j + ahead);
-        values(s1, j1);
-        scores(s1, j1 + ahead);
+      constexpr int AHEAD = NQ == 2 ? 1 : 2;                 // key tiles that the scores are ahead of the values
+      // A poll costs about 100 cycles even when it finds what it waits for.  The MMAs of 64 dims take little longer, so
+      // their step waits for all that it needs and then issues both products in one go (64 heads over 4,096 tokens:
+      // 215 us for 233); those of 128 dims start sooner with the keys waited for between the products (16,384 tokens:
+      // 1,704 us for 1,742), and 256 dims have no third place for keys (2,048 behind 9,001: 237 us for 266).
+      constexpr bool GO = HD == 64;
+      auto step = [&](auto slot_c, int j) {
+        constexpr int slot = decltype(slot_c)::value;
+        if (!alive || j >= pl.tiles) return;
+        if (GO && slot == 0) need_k(j + 1);
+        if (NQ == 1 || slot == 0) need_v(j);
+        if (NQ == 1 || slot < slots) need(&p_full[slot], nullptr, NQ == 2 ? j : j >> 1);   // how often it was filled before
+        if (!alive) return;
+        umma::fence_after_sync();
+        if (one) {
+          values(slot_c, j);
+          if (GO && j + 1 < pl.tiles) scores(slot_c, j + 1);
+        }
+        __syncwarp();
+        if (GO || j + AHEAD >= pl.tiles) return;
+        if (NQ == 1 || slot == 0) need_k(j + AHEAD);
+        if (!alive) return;
+        umma::fence_after_sync();
+        if (one) scores(slot_c, j + AHEAD);
+        __syncwarp();
+      };
+      need(&q_full, &q_other, 0);
+      need_k(0);
+      if (alive) {
+        umma::fence_after_sync();
+        if (one) {
+          scores(s0, 0);
+          if (NQ == 2) scores(s1, 0);
+        }
+        __syncwarp();
+      }
+      if (NQ == 1 && pl.tiles > 1) {
+        need_k(1);
+        if (alive) {
+          umma::fence_after_sync();
+          if (one) scores(s1, 1);
+          __syncwarp();
+        }
+      }
+      for (int j = 0; j < pl.tiles && alive; j += AHEAD) {
+        step(s0, j);
+        step(s1, NQ == 2 ? j : j + 1);
       }
     }
   } else {
