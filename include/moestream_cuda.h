@@ -256,7 +256,7 @@ MS_API ms_status ms_model_batch_profile_step(ms_model* m, float* us, int max, in
  * rounded once to out_type.  Pairs: (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved.
  * in_type / out_type: f32, f16 or bf16.  An output may be its own input (same pointer, stride and type),
  * and must not overlap the inputs otherwise.  A token whose position is outside [0, max_pos) is not
- * written.  head_dim even and <= 512; n_tokens may be 0. */
+ * written.  head_dim even and <= 512, at most 65536 heads; n_tokens may be 0. */
 typedef struct ms_qk_rope {
   int n_tokens, heads, kv_heads, head_dim, rot_dim, interleaved;
   int in_type, out_type;
@@ -279,7 +279,7 @@ MS_API ms_status ms_qk_norm_rope(ms_ctx* ctx, const ms_qk_rope* args);
  * out = softmax(scale q k^T) v in f32 with the probabilities rounded to the element type for the second
  * product; a query without keys gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.
  * total_q / total_k: rows of q and out / of k and v (cu_q[n_seqs] and cu_k[n_seqs] at most).
- * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 128 per kv head; strides multiples of
+ * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 128 per kv head and 65536; strides multiples of
  * 8 elements, pointers 16-byte aligned; out must not overlap the inputs.  The values of v are finite. */
 typedef struct ms_prompt_attn {
   int n_seqs, heads, kv_heads, head_dim, type, window;

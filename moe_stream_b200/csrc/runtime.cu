@@ -14,6 +14,7 @@
 #include <unistd.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <cstdlib>
 #include <cstdarg>
 #include <cstdio>
@@ -1676,6 +1677,13 @@ namespace {
 
 bool elem_type(int t, bool f32) { return t == MS_Q_F16 || t == MS_Q_BF16 || (f32 && t == MS_Q_F32); }
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// int32 and f32 arrays (an address between two elements would fault)
+bool aligned_words(std::initializer_list<const void*> all) {
+  for (const void* p : all)
+    if (!aligned(p, 4)) return false;
+  return true;
+}
+constexpr int kMaxHeads = 65536;   // an offset inside a token's row fits 32 bits
 
 // the device of the context for one call; the caller's current device comes back
 struct OnDevice {
@@ -1692,6 +1700,7 @@ struct OnDevice {
 ms_status check_qk_rope(const ms_qk_rope& a, const char** why) {
   if (a.n_tokens < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.max_pos <= 0)
     return *why = "n_tokens >= 0, heads, kv_heads and max_pos > 0 required", MS_ERR_SHAPE;
+  if (a.heads > kMaxHeads || a.kv_heads > kMaxHeads) return *why = "at most 65536 heads", MS_ERR_SHAPE;
   if (a.head_dim <= 0 || a.head_dim % 2 || a.head_dim > 512 || a.rot_dim <= 0 || a.rot_dim % 2 || a.rot_dim > a.head_dim)
     return *why = "head_dim even and <= 512, rot_dim even and <= head_dim required", MS_ERR_SHAPE;
   if (!elem_type(a.in_type, true) || !elem_type(a.out_type, true))
@@ -1704,6 +1713,10 @@ ms_status check_qk_rope(const ms_qk_rope& a, const char** why) {
   if ((a.q_norm == nullptr) != (a.k_norm == nullptr)) return *why = "q_norm and k_norm go together", MS_ERR_INVALID_ARG;
   if (a.n_tokens && (!a.q || !a.k || !a.q_out || !a.k_out || !a.cos_t || !a.sin_t || !a.pos))
     return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
+  const size_t in = a.in_type == MS_Q_F32 ? 4 : 2, out = a.out_type == MS_Q_F32 ? 4 : 2;
+  if (!aligned(a.q, in) || !aligned(a.k, in) || !aligned(a.q_out, out) || !aligned(a.k_out, out) ||
+      !aligned_words({a.q_norm, a.k_norm, a.cos_t, a.sin_t, a.pos}))
+    return *why = "a pointer is not aligned to its elements", MS_ERR_SHAPE;
   if ((a.q_out == a.q && (a.q_out_stride != a.q_stride || a.in_type != a.out_type)) ||
       (a.k_out == a.k && (a.k_out_stride != a.k_stride || a.in_type != a.out_type)))
     if (a.n_tokens) return *why = "in place needs the input's stride and type", MS_ERR_INVALID_ARG;
@@ -1714,6 +1727,7 @@ ms_status check_prompt(const ms_prompt_attn& a, const char** why) {
   if (a.n_seqs < 0 || a.total_q < 0 || a.total_k < 0 || a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads)
     return *why = "counts >= 0 and heads a multiple of kv_heads required", MS_ERR_SHAPE;
   if (a.heads / a.kv_heads > 128) return *why = "at most 128 heads per kv head", MS_ERR_SHAPE;
+  if (a.heads > kMaxHeads) return *why = "at most 65536 heads", MS_ERR_SHAPE;
   if (((int64_t)a.total_q + a.n_seqs) * a.kv_heads > 0x3fffffffll) return *why = "too many rows", MS_ERR_SHAPE;
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return *why = "head_dim 64, 128 or 256 required", MS_ERR_SHAPE;
   if (!elem_type(a.type, false)) return *why = "f16 or bf16 required", MS_ERR_UNSUPPORTED_QTYPE;
@@ -1724,6 +1738,7 @@ ms_status check_prompt(const ms_prompt_attn& a, const char** why) {
     return *why = "strides must be multiples of 8 elements", MS_ERR_SHAPE;
   if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16))
     return *why = "pointers must be 16-byte aligned", MS_ERR_SHAPE;
+  if (!aligned_words({a.cu_q, a.cu_k, a.sinks})) return *why = "a pointer is not aligned to its elements", MS_ERR_SHAPE;
   if (!std::isfinite(a.scale) || a.scale < 0.0f) return *why = "scale > 0 (or 0 for the default) required", MS_ERR_INVALID_ARG;
   if (a.total_q && a.n_seqs && (!a.q || !a.out || !a.cu_q || !a.cu_k)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
   if (a.total_q && a.n_seqs && a.total_k && (!a.k || !a.v)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
@@ -1733,13 +1748,14 @@ ms_status check_prompt(const ms_prompt_attn& a, const char** why) {
 }
 
 ms_status check_cache(const ms_kv4_cache& c, const char** why) {
-  if (c.kv_heads <= 0 || c.kv_heads > 65536 || c.n_pages < 0 || c.n_seqs < 0 || c.max_pages < 0)
+  if (c.kv_heads <= 0 || c.kv_heads > kMaxHeads || c.n_pages < 0 || c.n_seqs < 0 || c.max_pages < 0)
     return *why = "kv_heads in 1 .. 65536 and counts >= 0 required", MS_ERR_SHAPE;
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return *why = "head_dim 64, 128 or 256 required", MS_ERR_SHAPE;
   if (c.page_tokens < 16 || c.page_tokens > 1024 || (c.page_tokens & (c.page_tokens - 1)))
     return *why = "page_tokens must be a power of two in 16 .. 1024", MS_ERR_SHAPE;
   if ((int64_t)c.max_pages * c.page_tokens > 0x7fff0000ll) return *why = "too many tokens per sequence", MS_ERR_SHAPE;
-  if (!aligned(c.pages, 16)) return *why = "pages must be 16-byte aligned", MS_ERR_SHAPE;
+  if (!aligned(c.pages, 16) || !aligned_words({c.block_table}))
+    return *why = "pages must be 16-byte aligned, block_table to its elements", MS_ERR_SHAPE;
   if ((c.n_pages && !c.pages) || (c.n_seqs && c.max_pages && !c.block_table))
     return *why = "pages or block_table missing", MS_ERR_INVALID_ARG;
   return MS_OK;
@@ -1753,7 +1769,8 @@ ms_status check_rows(const ms_kv4_cache& c, const ms_kv4_rows& r, const char** w
   const int64_t k = (int64_t)c.kv_heads * c.head_dim;
   if (r.k_stride < k || r.v_stride < k || r.k_stride % 8 || r.v_stride % 8)
     return *why = "strides must be multiples of 8 elements and hold a token's heads", MS_ERR_SHAPE;
-  if (!aligned(r.k, 16) || !aligned(r.v, 16)) return *why = "k and v must be 16-byte aligned", MS_ERR_SHAPE;
+  if (!aligned(r.k, 16) || !aligned(r.v, 16) || !aligned_words({r.cu, r.start}))
+    return *why = "k and v must be 16-byte aligned, cu and start to their elements", MS_ERR_SHAPE;
   if (r.total && c.n_seqs && (!r.cu || !r.start || !r.k || !r.v)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
   return MS_OK;
 }
@@ -1778,6 +1795,7 @@ ms_status check_kv4_attn(const ms_kv4_cache& c, const ms_kv4_attn& a, const char
   if (!std::isfinite(a.scale) || a.scale < 0.0f) return *why = "scale > 0 (or 0 for the default) required", MS_ERR_INVALID_ARG;
   if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.work, 16))
     return *why = "pointers must be 16-byte aligned", MS_ERR_SHAPE;
+  if (!aligned_words({a.lens, a.sinks})) return *why = "a pointer is not aligned to its elements", MS_ERR_SHAPE;
   if (c.n_seqs && (!a.q || !a.out || !a.lens || !a.work)) return *why = "a pointer is missing", MS_ERR_INVALID_ARG;
   if (c.n_seqs && a.out == a.q) return *why = "out must not overlap q", MS_ERR_INVALID_ARG;
   return MS_OK;

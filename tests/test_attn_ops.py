@@ -30,6 +30,7 @@ def make(cls, **kw):
 ROPE = dict(n_tokens=3, heads=8, kv_heads=2, head_dim=128, rot_dim=64, in_type=0, out_type=30, eps=1e-6, max_pos=10, q=P,
             k=P, q_stride=1024, k_stride=256, q_norm=P, k_norm=P, cos_t=P, sin_t=P, pos=P, q_out=2 * P, k_out=2 * P,
             q_out_stride=1024, k_out_stride=256)
+ROPE_BIG = dict(q_stride=1 << 40, k_stride=1 << 40, q_out_stride=1 << 40, k_out_stride=1 << 40)
 PROMPT = dict(n_seqs=2, heads=8, kv_heads=2, head_dim=64, type=30, total_q=10, total_k=20, q=P, k=P, v=P, q_stride=512,
               k_stride=128, v_stride=128, cu_q=P, cu_k=P, out=2 * P, out_stride=512)
 CACHE = dict(kv_heads=2, head_dim=128, page_tokens=16, n_pages=5, pages=P, block_table=P, n_seqs=2, max_pages=3)
@@ -61,6 +62,35 @@ def test_rope_refusals(L, change, status):
 ], ids=str)
 def test_prompt_refusals(L, change, status):
     assert L.ms_prompt_attention(None, C.byref(make(_lib.PromptAttn, **{**PROMPT, **change}))) == status
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=P + 1), dict(k_out=P + 1), dict(in_type=1, k=P + 1), dict(out_type=0, q_out=P + 2), dict(q_norm=P + 2), dict(cos_t=P + 1),
+    dict(sin_t=P + 2), dict(pos=P + 2), dict(n_tokens=1, heads=65537, **ROPE_BIG), dict(n_tokens=1, kv_heads=1 << 24, **ROPE_BIG),
+], ids=str)
+def test_rope_addresses_between_elements_and_row_offsets(L, change):
+    assert L.ms_qk_norm_rope(None, C.byref(make(_lib.QkRope, **{**ROPE, **change}))) == SHAPE
+    fine = {k: v // 4 * 4 if k not in ("heads", "kv_heads") else 65536 for k, v in change.items() if not k.endswith("_type")}
+    assert L.ms_qk_norm_rope(None, C.byref(make(_lib.QkRope, **{**ROPE, **fine}))) == INVALID
+
+
+@pytest.mark.parametrize("change", [dict(cu_q=P + 2), dict(cu_k=P + 1), dict(sinks=P + 2),
+                                    dict(heads=131072, kv_heads=65536, q_stride=1 << 30, out_stride=1 << 30, k_stride=1 << 30, v_stride=1 << 30)], ids=str)
+def test_prompt_addresses_between_elements_and_row_offsets(L, change):
+    assert L.ms_prompt_attention(None, C.byref(make(_lib.PromptAttn, **{**PROMPT, **change}))) == SHAPE
+
+
+@pytest.mark.parametrize("name", ["block_table", "cu", "start", "lens", "sinks"])
+def test_cache_addresses_between_elements(L, name):
+    def calls(at):
+        c = make(_lib.Kv4CacheArgs, **{**CACHE, **({name: at} if name in CACHE else {})})
+        r = make(_lib.Kv4Rows, **{**ROWS, **({name: at} if name in ROWS else {})})
+        a = make(_lib.Kv4Attn, **{**ATTN, **({name: at} if name in ("lens", "sinks") else {})})
+        rows = [L.ms_kv4_write(None, C.byref(c), C.byref(r)), L.ms_kv4_read(None, C.byref(c), C.byref(r))]
+        attn = [L.ms_kv4_attention(None, C.byref(c), C.byref(a))]
+        return rows + attn if name in CACHE else rows if name in ROWS else attn
+    assert set(calls(P + 2)) == {SHAPE}
+    assert set(calls(P + 4)) == {INVALID}                             # fine but for the context
 
 
 CACHE_BAD = [(dict(kv_heads=0), SHAPE), (dict(kv_heads=70000), SHAPE), (dict(head_dim=96), SHAPE), (dict(page_tokens=8), SHAPE), (dict(page_tokens=48), SHAPE),
