@@ -6,11 +6,14 @@ point raises.  Build it with ``python -m moe_stream_b200.build``.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import re
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_build", "libmoestream_cuda.so")
+BINDING_PATH = os.path.join(HERE, "_build", "_binding.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "moestream_cuda.h")
 
 MS_OK = 0
@@ -206,6 +209,25 @@ def lib() -> C.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The extension that reads torch tensors and calls the library's attention operators (csrc/binding.cpp)."""
+    global _binding
+    if _binding is None:
+        if not os.path.exists(BINDING_PATH):
+            raise OSError(f"{BINDING_PATH} is missing: build it with `python -m moe_stream_b200.build`")
+        import torch  # noqa: F401  (loads the libraries that the extension needs)
+        loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+        loader.exec_module(m)
+        m.entries(*(C.cast(getattr(lib(), f"ms_{n}"), C.c_void_p).value
+                    for n in ("qk_norm_rope", "prompt_attention", "kv4_write", "kv4_read", "kv4_attention")))
+        _binding = m
+    return _binding
 
 
 def check(status: int, ctx=None) -> None:

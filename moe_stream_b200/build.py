@@ -1,10 +1,11 @@
 """Build libmoestream_cuda (shared, for ctypes / FFI callers, and static, for a Rust build.rs)
-in-tree under moe_stream_b200/_build/ with nvcc for sm_100a.  Run: python -m moe_stream_b200.build"""
+in-tree under moe_stream_b200/_build/ with nvcc for sm_100a, and the extension that reads torch tensors.  Run: python -m moe_stream_b200.build"""
 from __future__ import annotations
 
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -16,6 +17,7 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
 SO = os.path.join(OUT, "libmoestream_cuda.so")
 A = os.path.join(OUT, "libmoestream_cuda.a")
+BINDING = os.path.join(OUT, "_binding.so")
 
 
 def _stale(target: str, deps) -> bool:
@@ -36,7 +38,14 @@ def build(verbose: bool = False) -> str:
         if _stale(o, [s] + headers):
             cmds.append([NVCC, *FLAGS, "-c", s, "-o", o])
         objs.append(o)
-    # translation units compile in parallel (one nvcc process each)
+    src = os.path.join(CSRC, "binding.cpp")
+    if _stale(BINDING, [src, headers[-1]]):
+        import torch
+        at = os.path.dirname(torch.__file__)
+        cmds.append(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-isystem", os.path.join(at, "include"),
+                     "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING, "-L" + os.path.join(at, "lib"), "-lc10",
+                     "-ltorch_cpu", "-ltorch_python"])
+    # translation units compile in parallel (one compiler process each)
     procs = []
     for cmd in cmds:
         if verbose:

@@ -10,14 +10,13 @@ the CUDA library; nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes as C
-import struct
 import weakref
 from typing import Optional, Sequence
 
 import numpy as np
 
 from . import gguf as G
-from ._lib import ARCH_GPT_OSS, ARCH_QWEN_MOE, ModelConfig, check, lib
+from ._lib import ARCH_GPT_OSS, ARCH_QWEN_MOE, ModelConfig, binding, check, lib
 
 
 def _ptr(t) -> int:
@@ -26,58 +25,6 @@ def _ptr(t) -> int:
         return None
     if isinstance(t, int):
         return t
-    return t.data_ptr()
-
-
-# ---- arguments of the attention operators: torch tensors are looked at, checked and packed into the C structs.  A
-# decode step makes several of these calls per layer, so they are written for few Python operations. ----
-_PACK_ROPE = struct.Struct("@8ifi2P2q7P2q").pack
-_PACK_PROMPT = struct.Struct("@8if3P3q4Pq").pack
-_PACK_ROWS = struct.Struct("@2i4P2q").pack
-_PACK_ATTN = struct.Struct("@4if5PN").pack
-_TYPE_IDS: dict = {}   # torch dtype -> MS_Q_* element type, and "i32" -> torch.int32, "f32" -> torch.float32
-
-
-def _type_id(t) -> int:
-    i = _TYPE_IDS.get(t.dtype)
-    if i is None:
-        i = _TYPE_IDS[t.dtype] = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 30}.get(str(t.dtype), -1)
-    return i
-
-
-def _is(t, name: str) -> bool:
-    """Whether a tensor has that dtype (torch itself is not imported here)."""
-    d = _TYPE_IDS.get(name)
-    if d is None:
-        if str(t.dtype) != name:
-            return False
-        d = _TYPE_IDS[name] = t.dtype
-    return t.dtype is d
-
-
-def _rows(what: str, t, heads: int, head_dim: int, n: int) -> int:
-    """Stride between the tokens of a [n, heads, head_dim] tensor whose heads are contiguous."""
-    if t.shape != (n, heads, head_dim):
-        raise ValueError(f"{what}: shape {tuple(t.shape)} is not [{n}, {heads}, {head_dim}]")
-    s0, s1, s2 = t.stride()
-    if n and ((s1 != head_dim and heads > 1) or (s2 != 1 and head_dim > 1)):
-        raise ValueError(f"{what}: the heads of a token must be contiguous (strides {tuple(t.stride())})")
-    return s0 if n > 1 else heads * head_dim
-
-
-def _index(what: str, t, n: int) -> int:
-    """Device pointer of a contiguous int32 vector [n]."""
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or not _is(t, "torch.int32"):
-        raise ValueError(f"{what}: a contiguous int32 tensor of {n} values is needed, got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
-
-
-def _floats(what: str, t, n: int) -> int:
-    """Device pointer of n contiguous f32 values, 0 for None."""
-    if t is None:
-        return 0
-    if t.numel() != n or not t.is_contiguous() or not _is(t, "torch.float32"):
-        raise ValueError(f"{what}: {n} contiguous f32 values are needed, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
@@ -93,7 +40,7 @@ class KV4Cache:
             raise ValueError(f"pages: a contiguous uint8 tensor of whole pages of {per} bytes is needed")
         if pages.device != block_table.device:
             raise ValueError("pages and block_table are on different devices")
-        if block_table.dim() != 2 or not block_table.is_contiguous() or not _is(block_table, "torch.int32"):
+        if block_table.dim() != 2 or not block_table.is_contiguous() or str(block_table.dtype) != "torch.int32":
             raise ValueError("block_table: a contiguous int32 tensor [sequences, pages per sequence] is needed")
         table = block_table.data_ptr()
         self.pages, self.block_table = pages, block_table
@@ -239,61 +186,37 @@ class Context:
                                      hidden, inter, _ptr(x), _ptr(y)), self.h)
 
     # ---- attention operators of ragged batches (torch tensors; shapes, strides and types are read from them) ----
-    def _here(self, *tensors) -> None:
-        for t in tensors:
-            if t is not None and t.get_device() != self.device:
-                raise ValueError(f"a tensor is on {t.device}, the context on cuda:{self.device}")
-
+    # The tensors are looked at in csrc/binding.cpp; what does not fit together is a ValueError.
     def qk_norm_rope(self, q, k, q_norm, k_norm, eps: float, cos, sin, pos, q_out, k_out,
                      interleaved: bool = False) -> None:
         """q_out / k_out = RoPE(RMSNorm(q / k)) per head: q [tokens, heads, hd], k [tokens, kv_heads, hd] (f32,
         f16 or bf16; the outputs' type may differ, and they may be the inputs), norm weights [hd] f32 (or
         both None), tables cos / sin [max_pos, rot_dim / 2] f32 indexed by pos [tokens] (int32)."""
-        self._here(q, k, q_norm, k_norm, cos, sin, pos, q_out, k_out)
-        n, H, hd = q.shape
-        kv = k.shape[1]
-        if q.dtype != k.dtype or q_out.dtype != k_out.dtype or cos.dim() != 2 or cos.shape != sin.shape:
-            raise ValueError("q and k, q_out and k_out, cos and sin go together")
-        rows, half = cos.shape
-        a = _PACK_ROPE(n, H, kv, hd, 2 * half, int(interleaved), _type_id(q), _type_id(q_out), eps, rows, q.data_ptr(),
-                       k.data_ptr(), _rows("q", q, H, hd, n), _rows("k", k, kv, hd, n), _floats("q_norm", q_norm, hd),
-                       _floats("k_norm", k_norm, hd), _floats("cos", cos, rows * half), _floats("sin", sin, rows * half),
-                       _index("pos", pos, n), q_out.data_ptr(), k_out.data_ptr(), _rows("q_out", q_out, H, hd, n),
-                       _rows("k_out", k_out, kv, hd, n))
-        check(lib().ms_qk_norm_rope(self.h, a), self.h)
+        st = binding().qk_norm_rope(self.h and self.h.value, self.device, q, k, q_norm, k_norm, eps, cos, sin, pos, q_out,
+                                    k_out, interleaved)
+        if st:
+            check(st, self.h)
 
     def prompt_attention(self, q, k, v, cu_q, cu_k, out, window: int = 0, sinks=None, scale: float = 0.0) -> None:
         """out = causal attention of packed sequences: q / out [total_q, heads, hd], k / v [total_k, kv_heads,
         hd] (f16 or bf16), cu_q / cu_k [sequences + 1] (int32), sinks [heads] f32; the last query of a
         sequence stands at its last key.  scale 0: 1 / sqrt(hd)."""
-        self._here(q, k, v, cu_q, cu_k, out, sinks)
-        n, H, hd = q.shape
-        m, kv, _ = k.shape
-        B = cu_q.shape[0] - 1
-        if not q.dtype == k.dtype == v.dtype == out.dtype:
-            raise ValueError("q, k, v and out must have one type")
-        a = _PACK_PROMPT(B, H, kv, hd, _type_id(q), window, n, m, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                         _rows("q", q, H, hd, n), _rows("k", k, kv, hd, m), _rows("v", v, kv, hd, m),
-                         _index("cu_q", cu_q, B + 1), _index("cu_k", cu_k, B + 1), _floats("sinks", sinks, H),
-                         out.data_ptr(), _rows("out", out, H, hd, n))
-        check(lib().ms_prompt_attention(self.h, a), self.h)
-
-    def _kv4_rows(self, cache: KV4Cache, k, v, cu, start):
-        self._here(cache.pages, k, v, cu, start)
-        n, kv, hd = k.shape[0], cache.kv_heads, cache.head_dim
-        if k.dtype != v.dtype:
-            raise ValueError("k and v must have one type")
-        return _PACK_ROWS(_type_id(k), n, _index("cu", cu, cache.n_seqs + 1), _index("start", start, cache.n_seqs),
-                          k.data_ptr(), v.data_ptr(), _rows("k", k, kv, hd, n), _rows("v", v, kv, hd, n))
+        st = binding().prompt_attention(self.h and self.h.value, self.device, q, k, v, cu_q, cu_k, out, window, sinks, scale)
+        if st:
+            check(st, self.h)
 
     def kv4_write(self, cache: KV4Cache, k, v, cu, start) -> None:
         """Quantise packed rows k / v [total, kv_heads, hd] (f32, f16 or bf16) into the cache: rows
         cu[i] .. cu[i + 1] become the tokens start[i], start[i] + 1, ... of sequence i."""
-        check(lib().ms_kv4_write(self.h, cache._ref, self._kv4_rows(cache, k, v, cu, start)), self.h)
+        st = binding().kv4_write(self.h and self.h.value, self.device, cache.pages, cache._ref, k, v, cu, start)
+        if st:
+            check(st, self.h)
 
     def kv4_read(self, cache: KV4Cache, cu, start, k, v) -> None:
         """The same rows read back from the cache into k / v."""
-        check(lib().ms_kv4_read(self.h, cache._ref, self._kv4_rows(cache, k, v, cu, start)), self.h)
+        st = binding().kv4_read(self.h and self.h.value, self.device, cache.pages, cache._ref, k, v, cu, start)
+        if st:
+            check(st, self.h)
 
     def kv4_attention_workspace_bytes(self, cache: KV4Cache, n_seqs: int, n_query: int, heads: int) -> int:
         """Bytes of the workspace that kv4_attention needs for that many sequences of the cache."""
@@ -307,15 +230,10 @@ class Context:
         """out = attention of q [sequences, n_query, heads, hd] (f16 or bf16, contiguous), the newest n_query
         of each sequence's lens[i] cached tokens; sinks [heads] f32.  work: a uint8 tensor of
         kv4_attention_workspace_bytes, of this call alone while it runs.  scale 0: 1 / sqrt(hd)."""
-        self._here(cache.pages, q, lens, out, work, sinks)
-        B, n, H, hd = q.shape
-        if B != cache.n_seqs or hd != cache.head_dim or q.shape != out.shape or q.dtype != out.dtype:
-            raise ValueError(f"q and out must be [{cache.n_seqs}, n_query, heads, {cache.head_dim}] of one type")
-        if not (q.is_contiguous() and out.is_contiguous() and work.is_contiguous()):
-            raise ValueError("q, out and work must be contiguous")
-        a = _PACK_ATTN(n, H, _type_id(q), window, scale, q.data_ptr(), _index("lens", lens, B), _floats("sinks", sinks, H),
-                       out.data_ptr(), work.data_ptr(), work.numel() * work.element_size())
-        check(lib().ms_kv4_attention(self.h, cache._ref, a), self.h)
+        st = binding().kv4_attention(self.h and self.h.value, self.device, cache.pages, cache._ref, q, lens, out, work, window,
+                                     sinks, scale)
+        if st:
+            check(st, self.h)
 
     def close(self) -> None:
         if getattr(self, "h", None):

@@ -154,3 +154,86 @@ def test_quantised_values_are_near(hd=128):
     d, o = d.astype(np.float64)[:, None], o.astype(np.float64)[:, None]
     err = np.abs(o + d * (16 + c) - x)
     assert (err <= d * (0.5 + 31 * 2.0 ** -11) + np.abs(o) * 2.0 ** -11).all()
+
+
+# ---------------------------------------------------------------- the binding: tensors on the CPU, no context behind it
+
+class Calls:
+    """The calls of a context without a device, with tensors that fit; a change replaces one."""
+
+    def __init__(self):
+        import torch
+        from moe_stream_b200 import Context, KV4Cache
+        self.torch = torch
+        self.ctx = object.__new__(Context)
+        self.ctx.h, self.ctx.device = None, -1                        # CPU tensors are on device -1
+        bf, i32 = torch.bfloat16, torch.int32
+        z = torch.zeros
+        cache = KV4Cache(z(5 * KV4Cache.page_bytes(2, 64, 16), dtype=torch.uint8), z(3, 4, dtype=i32), 2, 64, 16)
+        rows = dict(cache=cache, k=z(7, 2, 64, dtype=bf), v=z(7, 2, 64, dtype=bf), cu=z(4, dtype=i32), start=z(3, dtype=i32))
+        self.args = {
+            "qk_norm_rope": dict(q=z(5, 8, 64), k=z(5, 2, 64), q_norm=z(64), k_norm=z(64), eps=1e-6, cos=z(9, 32), sin=z(9, 32),
+                                 pos=z(5, dtype=i32), q_out=z(5, 8, 64, dtype=bf), k_out=z(5, 2, 64, dtype=bf)),
+            "prompt_attention": dict(q=z(6, 8, 64, dtype=bf), k=z(9, 2, 64, dtype=bf), v=z(9, 2, 64, dtype=bf), cu_q=z(4, dtype=i32),
+                                     cu_k=z(4, dtype=i32), out=z(6, 8, 64, dtype=bf), window=3, sinks=z(8), scale=0.5),
+            "kv4_write": rows, "kv4_read": dict(rows),
+            "kv4_attention": dict(cache=cache, q=z(3, 1, 8, 64, dtype=bf), lens=z(3, dtype=i32), out=z(3, 1, 8, 64, dtype=bf),
+                                  work=z(64, dtype=torch.uint8), window=0, sinks=None, scale=0.0),
+        }
+
+    def call(self, name, **change):
+        return getattr(self.ctx, name)(**{**self.args[name], **change})
+
+
+@pytest.fixture(scope="module")
+def calls(L):
+    return Calls()
+
+
+@pytest.mark.parametrize("name", ["qk_norm_rope", "prompt_attention", "kv4_write", "kv4_read", "kv4_attention"])
+def test_binding_reaches_the_library(calls, name):
+    with pytest.raises(_lib.MsError) as e:                            # what fits is refused for want of a context alone
+        calls.call(name)
+    assert e.value.status == INVALID
+    calls.ctx.device = 0                                              # and for another device before that
+    with pytest.raises(ValueError, match="the context on cuda:0"):
+        calls.call(name)
+    calls.ctx.device = -1
+
+
+@pytest.mark.parametrize("name,arg,make", [
+    ("qk_norm_rope", "q", lambda t: t[:, :, :63]), ("qk_norm_rope", "q", lambda t: t[0]), ("qk_norm_rope", "k", lambda t: t.half()),
+    ("qk_norm_rope", "k", lambda t: t[:4]), ("qk_norm_rope", "q_norm", lambda t: t[:63]), ("qk_norm_rope", "k_norm", lambda t: t.double()),
+    ("qk_norm_rope", "cos", lambda t: t[:8]), ("qk_norm_rope", "sin", lambda t: t.t()), ("qk_norm_rope", "pos", lambda t: t.long()),
+    ("qk_norm_rope", "pos", lambda t: t[:4]), ("qk_norm_rope", "q_out", lambda t: t.float()), ("qk_norm_rope", "k_out", lambda t: t[:, :1]),
+    ("qk_norm_rope", "q", lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)),
+    ("prompt_attention", "k", lambda t: t[:8]), ("prompt_attention", "v", lambda t: t.half()), ("prompt_attention", "out", lambda t: t[:5]),
+    ("prompt_attention", "cu_q", lambda t: t[:3]), ("prompt_attention", "cu_k", lambda t: t.long()),
+    ("prompt_attention", "sinks", lambda t: t.bfloat16()), ("prompt_attention", "sinks", lambda t: t[::2]),
+    ("prompt_attention", "window", lambda w: 1 << 40), ("prompt_attention", "q", lambda t: t.transpose(1, 2)),
+    ("kv4_write", "k", lambda t: t[:6]), ("kv4_write", "v", lambda t: t.float()), ("kv4_read", "cu", lambda t: t[:3]),
+    ("kv4_read", "start", lambda t: t.float()), ("kv4_read", "k", lambda t: t.reshape(7, 128)),
+    ("kv4_attention", "q", lambda t: t[:2]), ("kv4_attention", "out", lambda t: t.half()), ("kv4_attention", "lens", lambda t: t[:2]),
+    ("kv4_attention", "q", lambda t: t[:, 0]), ("kv4_attention", "out", lambda t: t.transpose(2, 3).contiguous().transpose(2, 3)),
+])
+def test_binding_refuses_what_does_not_fit(calls, name, arg, make):
+    with pytest.raises(ValueError):
+        calls.call(name, **{arg: make(calls.args[name][arg])})
+
+
+@pytest.mark.parametrize("name,arg,value", [("qk_norm_rope", "q", None), ("prompt_attention", "cu_q", [0, 1]), ("kv4_write", "k", 4096),
+                                            ("kv4_attention", "work", "x"), ("prompt_attention", "scale", "y"), ("kv4_attention", "window", 1.5)])
+def test_binding_refuses_other_types(calls, name, arg, value):
+    with pytest.raises(TypeError):
+        calls.call(name, **{arg: value})
+
+
+def test_binding_takes_strided_rows_and_one_token(calls):
+    t = calls.torch
+    fused = t.zeros(5, 12 * 64)                                       # the fused projection's rows
+    q, k = fused[:, :512].view(5, 8, 64), fused[:, 512:640].view(5, 2, 64)
+    one = dict(q=q[:1], k=k[:1], pos=calls.args["qk_norm_rope"]["pos"][:1], q_out=t.zeros(1, 8, 64), k_out=t.zeros(1, 2, 64))
+    for change in (dict(q=q, k=k), one, dict(q_norm=None, k_norm=None), dict(interleaved=True)):
+        with pytest.raises(_lib.MsError) as e:
+            calls.call("qk_norm_rope", **change)
+        assert e.value.status == INVALID
