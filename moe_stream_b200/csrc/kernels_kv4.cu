@@ -5,7 +5,7 @@
 // attention kernel builds tensor-core operands from it with one mask-and-or.  The layout of a block of 16 tokens
 // is in include/moestream_cuda.h.  Both kernels are bound by memory: every row and every block byte moves once.
 // Reading 61,000 tokens of 4 heads of 128 dims (154 MB) takes 29 us, 5.3 TB/s; writing and reading back 8,900 tokens
-// of 8 heads of 64 dims 19 us, two launches and their look-ups before the 48 MB.
+// of 8 heads of 64 dims 17 us, two launches and their look-ups before the 48 MB.
 #include <type_traits>
 
 #include "../../include/moestream_cuda.h"
@@ -71,86 +71,113 @@ __device__ __forceinline__ void find_leads(const ms_kv4_cache& c, const ms_kv4_r
   __syncthreads();
 }
 
-// ---- quantising: 8 dims of a group of 32 held by 4 neighbouring lanes ----
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+// ---- quantising: 8 dims of a group of 32 held by 4 neighbouring lanes (all lanes of a warp take part) ----
+// largest value and minus the smallest of two packed pairs' halves; NaN when there is one
+template <class T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  if (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// whether a value is beyond +-16384, infinite or NaN
 template <class T>
-__device__ __forceinline__ bool unusual(const Raw8<T>& r) {
-  const uint32_t m = max_u16x2(max_u16x2(r.u.x & 0x7FFF7FFFu, r.u.y & 0x7FFF7FFFu), max_u16x2(r.u.z & 0x7FFF7FFFu, r.u.w & 0x7FFF7FFFu));
-  const uint32_t most = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7400u : 0x4680u;   // 16384 in f16 / bf16
-  return (m & 0xFFFFu) > most || (m >> 16) > most;
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (std::is_same<T, __half>::value) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
-template <>
-__device__ __forceinline__ bool unusual<float>(const Raw8<float>& r) {
-  return !(fabsf(r.a.x) <= 16384.f && fabsf(r.a.y) <= 16384.f && fabsf(r.a.z) <= 16384.f && fabsf(r.a.w) <= 16384.f &&
-           fabsf(r.b.x) <= 16384.f && fabsf(r.b.y) <= 16384.f && fabsf(r.b.z) <= 16384.f && fabsf(r.b.w) <= 16384.f);
-}
-struct Group8 {
-  uint32_t scale;   // f16 d, f16 o
-  uint32_t c[8];    // 0x4B400000 + code
-};
-constexpr float kMagic = 12582912.f;   // 1.5 * 2^23, bits 0x4B400000: adding it rounds to an integer in the low bits
-template <class T>
-__device__ __forceinline__ Group8 quantise8(const Raw8<T>& raw) {
-  Group8 g;
-  float x[8];
-  raw.get(x);
-  if (unusual(raw)) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -16384.f), 16384.f);
-  }
-  float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
-  float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+__device__ __forceinline__ void range_of(const float (&x)[8], float& lo, float& hi) {
+  lo = fminf(min3(x[0], x[1], x[2]), min3(min3(x[3], x[4], x[5]), x[6], x[7]));
+  hi = fmaxf(max3(x[0], x[1], x[2]), max3(max3(x[3], x[4], x[5]), x[6], x[7]));
 #pragma unroll
   for (int m = 1; m <= 2; m <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
   }
-  // d and o are rounded to f16 first and the codes computed from the rounded values
-  const __half dh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+}
+// smallest and largest value of the group.  False when one of its values is beyond +-16384, infinite or NaN
+template <class T>
+__device__ __forceinline__ bool range_of(const Raw8<T>& raw, const float (&)[8], float& lo, float& hi) {
+  const uint32_t a = max2<T>(max2<T>(raw.u.x, raw.u.y), max2<T>(raw.u.z, raw.u.w));
+  const uint32_t b = min2<T>(min2<T>(raw.u.x, raw.u.y), min2<T>(raw.u.z, raw.u.w)) ^ 0x80008000u;
+  uint32_t m = max2<T>(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+  m = max2<T>(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max2<T>(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const float2 f = unpack2<T>(m);
+  hi = f.x;
+  lo = -f.y;
+  return hi <= 16384.f && lo >= -16384.f;
+}
+__device__ __forceinline__ bool range_of(const Raw8<float>&, const float (&x)[8], float& lo, float& hi) {
+  range_of(x, lo, hi);
+  float sum = 0.f;                         // NaN when one is
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf(x[i], 0.f, sum);
+  return hi <= 16384.f && lo >= -16384.f && sum == 0.f;
+}
+struct Group8 {
+  uint32_t scale;   // f16 d, f16 o
+  uint64_t t[4];    // the codes as pairs of f32
+};
+constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
+// About 110 instructions for 8 values of each lane; one after the other, with the division, they were 200 and the kernel's bound.
+template <class T>
+__device__ __forceinline__ Group8 quantise8(const Raw8<T>& raw) {
+  Group8 g;
+  float x[8], lo, hi;
+  raw.get(x);
+  if (__any_sync(0xffffffffu, !range_of(raw, x, lo, hi))) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -16384.f), 16384.f);
+    range_of(x, lo, hi);
+  }
+  // d and o are rounded to f16 first and the codes computed from the rounded values.  The division by 15 is the product
+  // with its rounded reciprocal and Markstein's correction, which rounds it correctly (true for each of the 2^23 significands)
+  constexpr float k15 = 1.f / 15.f;
+  const float span = __fsub_rn(hi, lo), q = __fmul_rn(span, k15);
+  const __half dh = __float2half_rn(fmaf(fmaf(-15.f, q, span), k15, q));
   const float d = __half2float(dh);
-  const __half oh = __float2half_rn(__fsub_rn(lo, 16.0f * d));
+  const __half oh = __float2half_rn(fmaf(-16.f, d, lo));     // 16 d is exact
   const float o = __half2float(oh);
   g.scale = __half_as_ushort(dh) | (uint32_t)__half_as_ushort(oh) << 16;
-  // rint((x - o) / d) - 16 by the reciprocal (off by less than 2^-17 here); within 2^-12 of a tie, by the division
-  const float rd = d > 0.f ? __frcp_rn(d) : 0.f;
+  // rint((x - o) / d) - 16, clamped to 0 .. 15, as the fifteenfold of a value clamped to 0 .. 1, by an approximate
+  // reciprocal: together off by less than 2^-16 here.  Within 2^-12 of a tie, by the division
+  float rd;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rd) : "f"(d));
+  rd = d > 0.f ? rd * k15 : 0.f;
+  const uint64_t o2 = pair(-o, -o), up = pair(kMagic, kMagic), down = pair(-kMagic, -kMagic), p15 = pair(15.f, 15.f), n15 = pair(-15.f, -15.f);
   float near = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fmaxf(fmaf(__fsub_rn(x[i], o), rd, -16.f), 0.f), 15.f), z = y + kMagic;
-    near = fmaxf(near, fabsf(y - (z - kMagic)));
-    g.c[i] = __float_as_uint(z);
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpair(add2(pair(x[2 * i], x[2 * i + 1]), o2));
+    const uint64_t y = pair(__saturatef(fmaf(v.x, rd, -16.f * k15)), __saturatef(fmaf(v.y, rd, -16.f * k15)));
+    g.t[i] = add2(fma2(y, p15, up), down);
+    const float2 e = unpair(fma2(y, n15, g.t[i]));
+    near = max3(near, fabsf(e.x), fabsf(e.y));
   }
   if (near > 0.5f - 0x1p-12f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      g.c[i] = __float_as_uint(fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], o), d)) - 16.0f, 0.f), 15.f) + kMagic);
+    for (int i = 0; i < 4; ++i) {
+      float t[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) t[e] = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[2 * i + e], o), d)) - 16.0f, 0.f), 15.f);
+      g.t[i] = pair(t[0], t[1]);
+    }
   }
   return g;
 }
-// sum of c[i] << shift[i]; the magic parts of the c add up to a constant modulo 2^32
+// codes 2 n + h at bits 4 n + 16 h
 __device__ __forceinline__ uint32_t k_word(const Group8& g) {
-  uint32_t w = 0, k = 0;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    w += g.c[2 * n] * (1u << (4 * n)) + g.c[2 * n + 1] * (1u << (4 * n + 16));
-    k += 0x4B400000u * (1u << (4 * n)) + 0x4B400000u * (1u << (4 * n + 16));
-  }
-  return w - k;
+  const uint64_t k16 = pair(16.f, 16.f);
+  const float2 w = unpair(add2(fma2(fma2(fma2(g.t[3], k16, g.t[2]), k16, g.t[1]), k16, g.t[0]), pair(kMagic, kMagic)));
+  return __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410);
 }
-// four codes of one token and four of its partner, as the two halves of a word
-__device__ __forceinline__ uint32_t v_word(const uint32_t* a, const uint32_t* b) {
-  uint32_t w = 0, k = 0;
-#pragma unroll
-  for (int n = 0; n < 4; ++n) {
-    w += a[n] * (1u << (4 * n)) + b[n] * (1u << (4 * n + 16));
-    k += 0x4B400000u * (1u << (4 * n)) + 0x4B400000u * (1u << (4 * n + 16));
-  }
-  return w - k;
+// codes 4 q .. 4 q + 3 in the low 16 bits
+template <int Q>
+__device__ __forceinline__ uint32_t v_quad(const Group8& g) {
+  const float2 w = unpair(fma2(g.t[2 * Q + 1], pair(256.f, 256.f), g.t[2 * Q]));
+  return __float_as_uint(fmaf(w.y, 16.f, w.x) + kMagic);
 }
 
 // A row's heads are laid over the threads in order, 8 dims a thread, so a block's threads run through its rows.
@@ -203,15 +230,15 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const ms_kv4_cache 
     if (any_two) {
       const Group8 g1 = quantise8(vr[1]);
       if (live && two) {
-        *reinterpret_cast<uint2*>(vc) = make_uint2(v_word(g0.c, g1.c), v_word(g0.c + 4, g1.c + 4));
+        *reinterpret_cast<uint2*>(vc) = make_uint2(__byte_perm(v_quad<0>(g0), v_quad<0>(g1), 0x5410), __byte_perm(v_quad<1>(g0), v_quad<1>(g1), 0x5410));
         if (t == 0)
           *reinterpret_cast<uint2*>(vs) = make_uint2(__byte_perm(g0.scale, g1.scale, 0x5410), __byte_perm(g0.scale, g1.scale, 0x7632));
       }
     }
     if (live && !two) {
       const int par = tok & 1;
-      vc[par] = (uint16_t)v_word(g0.c, g0.c);
-      vc[2 + par] = (uint16_t)v_word(g0.c + 4, g0.c + 4);
+      vc[par] = (uint16_t)v_quad<0>(g0);
+      vc[2 + par] = (uint16_t)v_quad<1>(g0);
       if (t == 0) {
         vs[par] = (uint16_t)g0.scale;
         vs[2 + par] = (uint16_t)(g0.scale >> 16);

@@ -198,6 +198,28 @@ def test_kv4_write_and_read(ctx, case):
     assert (out[0][n:] == 9.0).all() and (out[1][n:] == 9.0).all()
 
 
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("t", ["float32", "bfloat16", "float16"])
+def test_kv4_write_values_half_way_between_codes(ctx, t, hd):
+    """Groups from 0 to 30 steps with 15 intervals: every odd value is a tie, which goes to the even code."""
+    t = getattr(torch, t)
+    cache, raw, table = new_cache([48], 16, 2, hd, seed=3)
+    r = np.random.default_rng(4)
+    x = r.integers(0, 31, (48, 2, hd // 32, 32)).astype(np.float32)
+    x[..., 0], x[..., 1] = 0, 30
+    x = r.permuted(x, axis=-1) - r.integers(0, 31, (48, 2, hd // 32, 1))
+    x *= 2.0 ** r.integers(-9, 9, (48, 2, hd // 32, 1)).astype(np.float32)
+    if t == torch.float32:                                            # and values next to the ties
+        x = np.where(r.random(x.shape) < 0.5, x, np.nextafter(x, np.float32(1e9) * r.choice([-1, 1], x.shape), dtype=np.float32))
+    k = torch.from_numpy(x.reshape(48, 2, hd).astype(np.float32)).cuda().to(t)
+    v = k.flip(0).contiguous()
+    ctx.kv4_write(cache, k, v, i32([0, 48]), i32([0]))
+    ctx.sync()
+    for j in range(48):
+        R.put_token(raw, table, 0, j, 16, 2, hd, k[j].float().cpu().numpy(), v[j].float().cpu().numpy())
+    assert np.array_equal(cache.pages.cpu().numpy(), raw)
+
+
 @pytest.mark.parametrize("t", ["float32", "bfloat16", "float16"])
 def test_kv4_write_unusual_values(ctx, t):
     t = getattr(torch, t)
