@@ -1,5 +1,5 @@
 // attn_types.cuh — element types (f32, f16, bf16) of the attention operators: 8-element vector loads and
-// stores with f32 values in registers, pairs of f32, and the lookup of a packed row's sequence.
+// stores with f32 values in registers, and pairs of f32.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -116,18 +116,6 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   float r;
   asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-
-// the sequence i with cu[i] <= j < cu[i + 1] (cu ascending from 0), or -1 when j is behind the last one
-__device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seqs, int j) {
-  if (j >= cu[n_seqs]) return -1;
-  int lo = 0, hi = n_seqs - 1;   // the last i with cu[i] <= j
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= j) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
 }
 
 // Launch a kernel; a small grid may start while its predecessor in the stream ends (the kernel calls pdl_wait_prior

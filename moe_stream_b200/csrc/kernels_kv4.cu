@@ -36,18 +36,27 @@ __device__ __forceinline__ void find_leads(const ms_kv4_cache& c, const ms_kv4_r
     bool lead = false;
     int64_t block = 0;
     int tok = 0;
-    // the row's sequence: up to 32 sequences from one load, more by bisection
-    int i = -1, begin = 0, end = 0, first = 0;
-    if (c.n_seqs <= 32) {
-      const int lo = lane < c.n_seqs ? r.cu[lane] : 0x7fffffff, hi = lane < c.n_seqs ? r.cu[lane + 1] : 0, st = lane < c.n_seqs ? r.start[lane] : 0;
-      for (int s = 0; s < c.n_seqs; ++s) {
-        const int l = __shfl_sync(0xffffffffu, lo, s), h = __shfl_sync(0xffffffffu, hi, s), f = __shfl_sync(0xffffffffu, st, s);
-        if (l <= j && j < h) { i = s; begin = l; end = h; first = f; }
+    // the row's sequence, the last one that begins at or before it: from 32 samples of the offsets, one load, and among
+    // the sequences between two of them by bisection
+    const int stride = (c.n_seqs - 1) / 32 + 1, mine = lane * stride;
+    const bool have = mine < c.n_seqs;
+    const int lo = have ? r.cu[mine] : 0x7fffffff, hi = have && stride == 1 ? r.cu[mine + 1] : 0, st = have && stride == 1 ? r.start[mine] : 0;
+    int i = 0;
+    if (c.n_seqs > 1)
+#pragma unroll
+      for (int step = 16; step > 0; step >>= 1)
+        if (__shfl_sync(0xffffffffu, lo, i + step) <= j) i += step;
+    int begin = __shfl_sync(0xffffffffu, lo, i), end = __shfl_sync(0xffffffffu, hi, i), first = __shfl_sync(0xffffffffu, st, i);
+    if (stride > 1 && lane < rows) {
+      i *= stride;
+      for (int last = min(i + stride, c.n_seqs) - 1; i < last;) {
+        const int mid = (i + last + 1) >> 1;
+        if (r.cu[mid] <= j) i = mid;
+        else last = mid - 1;
       }
-    } else if (j < r.total) {
-      i = seq_of_row(r.cu, c.n_seqs, j);
-      if (i >= 0) { begin = r.cu[i]; end = r.cu[i + 1]; first = r.start[i]; }
+      begin = r.cu[i]; end = r.cu[i + 1]; first = r.start[i];
     }
+    if (j < begin || j >= end) i = -1;     // behind the last sequence
     if (lane < rows && j < r.total) {
       if (i >= 0) {
         const int at = j - begin, pos = first + at;
@@ -121,7 +130,8 @@ struct Group8 {
   uint64_t t[4];    // the codes as pairs of f32
 };
 constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
-// About 110 instructions for 8 values of each lane; one after the other, with the division, they were 200 and the kernel's bound.
+// The kernel executes 142 warp instructions for 8 values of each lane; with the values one by one and __fdiv_rn it were 201,
+// which bound it (write and read back 8,900 tokens of 8 heads of 64 dims: 19.0 us for 16.9).
 template <class T>
 __device__ __forceinline__ Group8 quantise8(const Raw8<T>& raw) {
   Group8 g;

@@ -161,6 +161,10 @@ CACHE = [  # new, start, page, kv, hd, type
     ([33, 2], [1, 30], 32, 1, 128, "bfloat16"),
     ([17, 18], [0, 63], 64, 3, 256, "float16"),
     ([2, 3, 4, 5, 6, 7], [1, 1, 2, 2, 3, 3], 128, 1, 64, "bfloat16"),
+    ([1] * 32, [5 * i % 33 for i in range(32)], 16, 1, 64, "float16"),
+    ([7 * i * i % 5 for i in range(77)], [3 * i % 19 for i in range(77)], 16, 1, 64, "float16"),
+    ([0] * 40 + [3] + [0] * 20 + [1], [2] * 62, 16, 2, 64, "bfloat16"),
+    ([2 + i % 2 for i in range(300)], [i % 3 for i in range(300)], 16, 1, 64, "bfloat16"),
 ]
 
 
