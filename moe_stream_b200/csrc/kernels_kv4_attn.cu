@@ -26,7 +26,7 @@
 // reduction over the lanes.
 //
 // Measured: 32 sequences of 8,300 tokens on average, 4 heads of 128 dims (162 MB): 43 us, 3.7 TB/s; one of 131,072
-// tokens, 8 heads of 64 dims (84 MB, f16): 29 us; one of 4,097 tokens: 9 us.  Bulk copies alone stream the first
+// tokens, 8 heads of 64 dims (84 MB, f16): 28 us; one of 4,097 tokens: 9 us.  Bulk copies alone stream the first
 // in 30 us; 3 us go by before the first copy (lengths, split, page numbers), the blocks end up to 4 us apart, and the
 // second kernel takes 3 to 4 us.  The loop issues 330 instructions a warp for 16 tokens of 128 dims and keeps the
 // issue slots half busy.
@@ -758,8 +758,8 @@ cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_attn& a, 
   cfg.gridDim = dim3(c.n_seqs * c.kv_heads * row_tiles, min(rows, 8 * NT));
   cfg.dynamicSmemBytes = 0;
   // Few jobs have many parts each, and one round of loads costs about a microsecond: 16 loads at a time then.  One
-  // sequence, 4 heads of 128 dims, 8 against 16: 7.6 / 7.6 us (200 tokens), 9.1 / 8.7 (4,097), 12.8 / 11.1 (9,000).  With many jobs the blocks' registers
-  // count: 32 sequences of 8,300 tokens on average 43.5 against 45.2 us.
+  // sequence, 4 heads of 128 dims, 8 against 16: 7.6 / 7.6 us (200 tokens), 9.1 / 8.7 (4,097), 12.8 / 11.1 (9,000).  With
+  // many jobs the blocks' registers count: 32 sequences of 8,300 tokens on average 43.5 against 45.2 us.
   if (ranges_of(d, HD, NT) >= 32 * (int)cfg.gridDim.x)
     return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, HD, NT, 16>, c, a, row_tiles, ranges_of(d, HD, NT));
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, HD, NT, 8>, c, a, row_tiles, ranges_of(d, HD, NT));
