@@ -1,7 +1,7 @@
 // binding.cpp — the attention operators' arguments from torch tensors.  A decode step makes several of these calls per
 // layer and the kernels behind them take a few microseconds; with the tensors looked at and packed in Python, calls of
-// one token's rotation followed each other after 8.3 us, with this after 2.9 (a decode step's write and read back: 12.1
-// and 6.3, both launches' own time).  The entry points come from the library that ctypes has loaded (`entries`), so there is one
+// one token's rotation followed each other after 8.3 us, with this after 2.6 (a decode step's write and read back: 12.1
+// and 5.7, nearly the launches' own time).  The entry points come from the library that ctypes has loaded (`entries`), so there is one
 // copy of it in the process.  What a call cannot take is a ValueError before anything is launched; the library's own
 // checks answer with their status.
 #include <Python.h>

@@ -131,7 +131,7 @@ struct Group8 {
 };
 constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
 // The kernel executes 142 warp instructions for 8 values of each lane; with the values one by one and __fdiv_rn it were 201,
-// which bound it (write and read back 8,900 tokens of 8 heads of 64 dims: 19.0 us for 16.9).
+// which bound it (write and read back 8,900 tokens of 8 heads of 64 dims: 19.0 us for 17.0).
 template <class T>
 __device__ __forceinline__ Group8 quantise8(const Raw8<T>& raw) {
   Group8 g;
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const ms_kv4_cache c
 template <class T, int HD>
 cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_rows& r, bool write, cudaStream_t s) {
   // 16 rows share a look-up, with few rows down to 2, so that a decode step spreads over the SMs (write and read back,
-  // 16 rows against 2: 16.8 / 6.0 us for 32 tokens, 21.8 / 24.6 for 8,900; in between the rule takes 4 or 8)
+  // 16 rows against 2: 15.0 / 5.1 us for 32 tokens, 19.5 / 22.3 for 8,900, where the rule takes 8: 17.0)
   int rows = kRows;
   while (rows > 2 && (int64_t)r.total < (int64_t)rows * 4 * d.sm_count) rows /= 2;
   const uint32_t grid = (uint32_t)(((int64_t)r.total + rows - 1) / rows);
