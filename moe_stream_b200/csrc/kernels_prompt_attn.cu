@@ -38,6 +38,7 @@
 #include "attn_types.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "phases.h"
 #include "umma.cuh"
 
 namespace ms {
@@ -484,6 +485,8 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < BN / 64; ++i) umma::st_32x32b_x32(p_col + 32 * i, u + 32 * i);
         umma::wait_st();
+        if (NQ == 1 && waits_before_handover(j, pl.tiles)) alive = wait(&o_full[0], j - 1);
+        if (!alive) break;
         umma::fence_before_sync();
         __syncwarp();
         if (lane == 0) {
@@ -493,8 +496,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
       }
       // ---- output ----
       // A wait on a phase's parity tells it from the one before only: the scores of tile j vouch for the value products
-      // up to j - 1 (NQ = 2) or j - 2, so with NQ = 1 the last but one is waited for first.
-      if (NQ == 1 && pl.tiles > 1 && alive) alive = wait(&o_full[0], pl.tiles - 2);
+      // up to j - 1 (NQ = 2) or j - 2, so with NQ = 1 the last but one was waited for before the last hand-over.
       if (pl.tiles > 0 && alive) alive = wait(&o_full[NQ == 2 ? tile : 0], pl.tiles - 1);
       umma::fence_after_sync();
       float f = 0.f;
