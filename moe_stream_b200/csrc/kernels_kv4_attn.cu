@@ -37,6 +37,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
+#include "phases.h"
 
 namespace ms {
 namespace {
@@ -211,6 +212,7 @@ struct Smem {
   float m[kWarps][8 * NT], l[kWarps][8 * NT];
   uint64_t full[kWarps][kStages];
   uint32_t have[kWarps][kStages];         // blocks of the tile that were copied
+  int issued[kWarps];                     // tiles that the warp has fetched
 };
 
 // what a warp keeps of a job
@@ -415,6 +417,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&sm.full[warp][s], 1);
+    sm.issued[warp] = 0;
     fence_mbar_init();
   }
   __syncwarp();
@@ -436,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     const bool want = lane < (one_page ? 1 : TT >> shift) && token < pre.s.len && token + c.page_tokens > pre.s.lo;
     return want ? c.block_table[(int64_t)pre.seq * c.max_pages + (token >> shift)] : -2;   // -2: not needed
   };
-  auto fetch = [&](int stage, int page) {
+  auto fetch = [&](int k, int page) {                        // the warp's tile number k
+    const int stage = k % kStages;
     const int head = row_tiles > 1 ? pre.job / row_tiles : pre.job;
     const bool ok = (unsigned)page < (unsigned)c.n_pages;
     if (page != -2 && !ok) atomicOr(err, EF_BAD_INDEX);
@@ -445,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     if (!one_page) have = __reduce_or_sync(0xffffffffu, have);
     if (lane == 0) {
       sm.have[warp][stage] = have;
+      sm.issued[warp] = k + 1;
       mbar_expect_tx(&sm.full[warp][stage], __popc(have) * BLK);
     }
     if (!one_page) __syncwarp();
@@ -462,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     } while (next < count && pre.tile >= pre.s.n && (next += kWarps) < count);
     if (next < count) page = look_up();
   };
-  auto fetch_next = [&](int stage) {
-    fetch(stage, page);
+  auto fetch_next = [&](int k) {
+    fetch(k, page);
     next += kWarps;
     step_next(kWarps);
   };
@@ -554,10 +559,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
     const int t_first = row0 / rep, t_last = min(rows - 1, row0 + ROWS - 1) / rep;
     const int hi_all = len - a.n_query + t_first, lo_all = a.window > 0 ? len - a.n_query + t_last - a.window + 1 : 0;
 
+    bool landed = true;
     for (int x = at + ((warp - at) & (kWarps - 1)); x < end; x += kWarps) {
       const int stage = used % kStages;
-      const bool landed = mbar_wait(&sm.full[warp][stage], (used / kStages) & 1, err, EF_TIMEOUT_FULL);
-      const uint32_t have = landed ? sm.have[warp][stage] : 0u;
+      landed = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][stage], fill_phase(used, kStages) & 1, err, EF_TIMEOUT_FULL));
+      if (!landed) break;
+      const uint32_t have = sm.have[warp][stage];
       const int key0 = (cur.s.first + cur.tile + x - at) * TT;
       if (key0 >= lo_all && key0 + TT - 1 <= hi_all && have == (1u << TB) - 1)
         take_tile<HD, NT, false, RESTS>(R, K, sm.stage[warp][stage], key0, len, window, have);
@@ -565,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
         take_tile<HD, NT, true, RESTS>(R, K, sm.stage[warp][stage], key0, len, window, have);
       ++used;
       __syncwarp();                                          // the stage is free
-      if (next < count) fetch_next(stage);
+      if (next < count) fetch_next(used + kStages - 1);      // the other stages are full or on their way
     }
 
     // ---- join the warps: all on the largest maximum, the upper half of them into the lower half ----
@@ -580,7 +587,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
           sm.l[warp][8 * n + 2 * t + i] = R.l[n][i];
         }
       }
-    __syncthreads();
+    // where a wait ran out the block leaves, when no copy is under way any more
+    if (__syncthreads_or(!landed)) {
+      for (; used < sm.issued[warp]; ++used) mbar_wait(&sm.full[warp][used % kStages], fill_phase(used, kStages) & 1, nullptr, 0);
+      return;
+    }
     // tile k of the product, rows g and g + 8: dims 2 k and 2 k + 1 of the lane's chunk
     auto place = [&](int r, int k) -> float2* {
       const int d = HD == 64 ? 8 * g + 2 * k : 128 * (k >> 3) + 16 * g + 2 * (k & 7);

@@ -17,4 +17,7 @@ namespace ms {
 // back.  True at the tile in front of whose hand-over that wait stands.
 MS_PHASES_FN bool waits_before_handover(int tile, int tiles) { return tile > 0 && tile + 1 == tiles; }
 
+// A ring of stages, filled and emptied in turn: fill k goes to stage k % stages and completes this phase of its barrier.
+MS_PHASES_FN int fill_phase(int k, int stages) { return k / stages; }
+
 }  // namespace ms

@@ -13,8 +13,10 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 def phases(tmp_path_factory):
     at = tmp_path_factory.mktemp("phases")
     src, so = at / "p.cpp", at / "p.so"
-    src.write_text('#include "phases.h"\nextern "C" int waits_before_handover(int j, int n) '
-                   '{ return ms::waits_before_handover(j, n); }\n')
+    src.write_text('#include "phases.h"\nextern "C" {'
+                   'int waits_before_handover(int j, int n) { return ms::waits_before_handover(j, n); }'
+                   'int fill_phase(int k, int n) { return ms::fill_phase(k, n); }'
+                   '}\n')
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I" + CSRC, str(src), "-o", str(so)], check=True)
     return C.CDLL(str(so))
 
@@ -91,3 +93,14 @@ def test_the_model_sees_a_wait_that_comes_too_late():
     assert "stuck" in explore(3, (late, late))
     none = softmax_programs(3, lambda j: False, [2])[0]     # and without it the last one's wait may pass early
     assert "early" in explore(3, (none, none))
+
+
+@pytest.mark.parametrize("stages", [1, 2, 4])
+def test_a_ring_waits_for_every_fill(phases, stages):
+    """After any number of fills of which any of the last `stages` have not landed, a wait for one passes exactly when it
+    has landed."""
+    for issued in range(1, 4 * stages + 1):
+        for k in range(max(0, issued - stages), issued):
+            for landed in (False, True):
+                count = sum(i % stages == k % stages for i in range(k)) + landed   # phases of that stage that are over
+                assert (count % 2 != phases.fill_phase(k, stages) % 2) == landed
