@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
   uint8_t *sq = sm, *sk = sq + NQ * S::Q_BYTES, *sv = sk + ST * S::KV_BYTES;
   // *_other (rank 0 of a pair): the other block's share has arrived, too
   __shared__ uint64_t q_full, q_other, k_full[ST], k_other[ST], k_empty[ST], v_full[ST], v_other[ST], v_empty[ST], s_full[2], p_full[2],
-      o_full[NQ];
+      o_full[NQ], ended;
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CL == 2 ? cluster_rank() : 0, index = blockIdx.x / CL;
@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4 * CL); }
     for (int i = 0; i < NQ; ++i) mbar_init(&o_full[i], 1);
+    mbar_init(&ended, 1);
     fence_mbar_init();
   }
   pdl_wait_prior();
@@ -262,11 +263,10 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
             for (int b = 0; b < BLK; ++b)
               tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + (i * CL + rank) * n_tok, &q_full);
         }
-        bool alive = true;
-        for (int j = 0; j < pl.tiles; ++j) {
+        int j = 0;
+        for (; j < pl.tiles; ++j) {
           const int st = j % ST, z = pl.k0 + (pl.first + j) * BN;
-          if (j >= ST) alive = mbar_wait(&empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY);
-          if (!alive) break;
+          if (j >= ST && !mbar_wait(&empty[st], (j / ST - 1) & 1, err, EF_TIMEOUT_EMPTY)) break;
           mbar_expect_tx(&full[st], S::KV_BYTES);
           if (role == 1) {
             for (int b = 0; b < BLK; ++b)
@@ -276,11 +276,9 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
               tma_3d(sv + st * S::KV_BYTES + b * BN * 128, &v_map, 64 * (rank * S::V_BLOCKS + b), head, z, &full[st]);
           }
         }
-        // nothing of this block may still be on its way when it ends (the copies of an unfinished walk, too)
-        if (!alive) {
-          if (role == 1) mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
-          for (int i = 0; i < ST; ++i) mbar_wait(&full[i], 0, nullptr, 0);
-        }
+        // nothing of this block may still be on its way when it ends, also where another warp has given up
+        if (role == 1) mbar_wait(&q_full, 0, err, EF_TIMEOUT_FULL);
+        for (int k = first_under_way(j, ST); k < j; ++k) mbar_wait(&full[k % ST], fill_phase(k, ST) & 1, err, EF_TIMEOUT_FULL);
       }
     } else if (rank == 1) {
       // ---- the other block of a pair: Q and K, or V ----
@@ -290,7 +288,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
         if (alive && lane == 0) arrive_at_first(&q_other);
       }
       for (int j = 0; j < pl.tiles && alive; ++j) {
-        alive = wait(role == 0 ? &k_full[j % ST] : &v_full[j % ST], j / ST);
+        alive = wait(role == 0 ? &k_full[j % ST] : &v_full[j % ST], fill_phase(j, ST));
         if (!alive) break;
         if (role == 3 && clear_tail(j)) fence_cluster();
         if (lane == 0) arrive_at_first(role == 0 ? &k_other[j % ST] : &v_other[j % ST]);
@@ -307,10 +305,10 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
         alive = alive && wait(bar, parity) && (CL == 1 || bar_other == nullptr || wait(bar_other, parity));
       };
       auto need_k = [&](int j) {
-        if (j < pl.tiles) need(&k_full[j % ST], &k_other[j % ST], j / ST);
+        if (j < pl.tiles) need(&k_full[j % ST], &k_other[j % ST], fill_phase(j, ST));
       };
       auto need_v = [&](int j) {
-        need(&v_full[j % ST], &v_other[j % ST], j / ST);
+        need(&v_full[j % ST], &v_other[j % ST], fill_phase(j, ST));
         if (alive && clear_tail(j) && CL == 2) fence_cluster();
       };
       auto scores = [&](auto slot_c, int j) {                // one thread; K of tile j has arrived
@@ -390,6 +388,11 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
       for (int j = 0; j < pl.tiles && alive; j += AHEAD) {
         step(s0, j);
         step(s1, NQ == 2 ? j : j + 1);
+      }
+      if (pl.tiles > 0 && !alive) {                          // a wait ran out: the products under way end before the block does
+        if (one) umma::commit_here<CL>(&ended);
+        __syncwarp();
+        wait(&ended, 0);
       }
     }
   } else {

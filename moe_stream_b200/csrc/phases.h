@@ -19,5 +19,7 @@ MS_PHASES_FN bool waits_before_handover(int tile, int tiles) { return tile > 0 &
 
 // A ring of stages, filled and emptied in turn: fill k goes to stage k % stages and completes this phase of its barrier.
 MS_PHASES_FN int fill_phase(int k, int stages) { return k / stages; }
+// The first of so many fills that may be under way still: a stage is filled again when its last fill has been used.
+MS_PHASES_FN int first_under_way(int fills, int stages) { return fills > stages ? fills - stages : 0; }
 
 }  // namespace ms

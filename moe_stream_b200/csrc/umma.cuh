@@ -207,6 +207,14 @@ __device__ __forceinline__ void commit_cg(uint64_t* bar) {
                  : "memory");
 }
 
+// the same for the mbarrier of this block alone
+template <int CG>
+__device__ __forceinline__ void commit_here(uint64_t* bar) {
+  const uint32_t b = (uint32_t)__cvta_generic_to_shared(bar);
+  if constexpr (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b) : "memory");
+  else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b) : "memory");
+}
+
 // 32 lanes x 32 columns, without the wait (wait_ld before the values are used)
 __device__ __forceinline__ void ld_32x32b_x32_async(uint32_t taddr, uint32_t* r) {
   asm volatile(

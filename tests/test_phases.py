@@ -16,6 +16,7 @@ def phases(tmp_path_factory):
     src.write_text('#include "phases.h"\nextern "C" {'
                    'int waits_before_handover(int j, int n) { return ms::waits_before_handover(j, n); }'
                    'int fill_phase(int k, int n) { return ms::fill_phase(k, n); }'
+                   'int first_under_way(int k, int n) { return ms::first_under_way(k, n); }'
                    '}\n')
     subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I" + CSRC, str(src), "-o", str(so)], check=True)
     return C.CDLL(str(so))
@@ -98,9 +99,10 @@ def test_the_model_sees_a_wait_that_comes_too_late():
 @pytest.mark.parametrize("stages", [1, 2, 4])
 def test_a_ring_waits_for_every_fill(phases, stages):
     """After any number of fills of which any of the last `stages` have not landed, a wait for one passes exactly when it
-    has landed."""
+    has landed (a wait for parity 0 would pass at once where the fill under way is an odd one)."""
     for issued in range(1, 4 * stages + 1):
-        for k in range(max(0, issued - stages), issued):
+        assert phases.first_under_way(issued, stages) == max(0, issued - stages)
+        for k in range(phases.first_under_way(issued, stages), issued):
             for landed in (False, True):
                 count = sum(i % stages == k % stages for i in range(k)) + landed   # phases of that stage that are over
                 assert (count % 2 != phases.fill_phase(k, stages) % 2) == landed
