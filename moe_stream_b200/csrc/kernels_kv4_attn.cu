@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
   auto look_up = [&]() {
     const int token = (pre.s.first + pre.tile) * TT + (one_page ? 0 : lane << shift);
     const bool want = lane < (one_page ? 1 : TT >> shift) && token < pre.s.len && token + c.page_tokens > pre.s.lo;
-    return want ? c.block_table[(int64_t)pre.seq * c.max_pages + (token >> shift)] : -2;   // -2: not needed
+    return want ? max(c.block_table[(int64_t)pre.seq * c.max_pages + (token >> shift)], -1) : -2;   // -2: not needed
   };
   auto fetch = [&](int k, int page) {                        // the warp's tile number k
     const int stage = k % kStages;

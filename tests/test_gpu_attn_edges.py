@@ -40,3 +40,23 @@ def test_prompt_attention_ends_of_short_walks_beside_other_work(ctx, hd):
     for _, first, outs in sets:
         assert all(torch.equal(o, first) for o in outs)
     c2.close()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("entry", [-1, -2, -3, -2 ** 31, 2 ** 31 - 1])
+def test_kv4_attention_reports_every_bad_page_number(ctx, page, entry):
+    """The entry of a page that is attended; the result is the attention of the tokens that are there (half a step of bf16, and
+    2^-11 of p and of v and the scores' errors, together below 2^-8 of A)."""
+    from moe_stream_b200._lib import MsError
+    case = ([4 * page], 1, page, 8, 1, 64, 0, False, "bfloat16")
+    cache, table, q, lens, out, work, _, _ = G.cached_case(ctx, case, poison=False)
+    raw = cache.pages.cpu().numpy()
+    k, v = (torch.from_numpy(x).cuda() for x in R.cache_values(raw, table, 0, 4 * page, page, 1, 64)[:2])
+    keep = [j for j in range(4 * page) if j // page != 2]
+    cache.block_table[0, 2] = entry
+    ctx.kv4_attention(cache, q, lens, out, work)
+    with pytest.raises(MsError) as e:
+        ctx.sync()
+    assert e.value.status == 11
+    want, A = R.attention(q[0], k[keep], v[keep], torch.tensor([4 * page], device="cuda"), 0, 0.125, None)
+    G.within(out[0], want, 2.0 ** -8 * want.abs() + 2.0 ** -8 * A)
