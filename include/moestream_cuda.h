@@ -278,7 +278,8 @@ MS_API ms_status ms_qk_norm_rope(ms_ctx* ctx, const ms_qk_rope* args);
  * j > p - window when window > 0; sinks [heads] (f32, or NULL) join the softmax denominator.
  * out = softmax(scale q k^T) v in f32 with the probabilities rounded to the element type for the second
  * product; a query without keys gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.
- * total_q / total_k: rows of q and out / of k and v (cu_q[n_seqs] and cu_k[n_seqs] at most).
+ * total_q / total_k: rows of q and out / of k and v (cu_q[n_seqs] and cu_k[n_seqs] at most).  Offsets that descend, are
+ * negative or end behind these are reported (MS_ERR_DEVICE_INDEX); out then holds nothing of use for any sequence.
  * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 128 per kv head and 65536; strides multiples of
  * 8 elements, pointers 16-byte aligned; out must not overlap the inputs.  The values of v are finite. */
 typedef struct ms_prompt_attn {
@@ -317,8 +318,9 @@ MS_API ms_status ms_kv4_page_bytes(int kv_heads, int head_dim, int page_tokens, 
 
 /* Quantise packed rows k / v [total][kv_heads][head_dim] (f32, f16 or bf16) into the cache, or read the
  * cache back into them (rounded once from f32): rows cu[i] .. cu[i + 1] are the tokens start[i],
- * start[i] + 1, ... of sequence i.  Rows behind cu[n_seqs] are skipped.  Writing touches the bytes of its own
- * tokens only; two calls that write the same token at the same time leave either. */
+ * start[i] + 1, ... of sequence i.  Rows behind cu[n_seqs] are skipped.  Offsets that descend, are negative or end
+ * behind `total` are reported (MS_ERR_DEVICE_INDEX); which of the sequences' tokens and rows were taken then is open.
+ * Writing touches the bytes of its own tokens only; two calls that write the same token at the same time leave either. */
 typedef struct ms_kv4_rows {
   int type, total;
   const int32_t *cu, *start;   /* [n_seqs + 1] ascending from 0, [n_seqs] (device) */

@@ -1,5 +1,5 @@
 // attn_types.cuh — element types (f32, f16, bf16) of the attention operators: 8-element vector loads and
-// stores with f32 values in registers, and pairs of f32.
+// stores with f32 values in registers, pairs of f32, and a check of packed sequences' offsets.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -116,6 +116,17 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   float r;
   asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// One warp's share, 32 of every `step` sequences from `first` on, of the check of offsets cu [n_seqs + 1]: false in a lane
+// that sees a negative or descending one, or an end behind `total`.
+__device__ __forceinline__ bool offsets_ok(const int32_t* cu, int n_seqs, int total, int first, int step) {
+  bool ok = true;
+  for (int i = first + (threadIdx.x & 31); i < n_seqs; i += step) {
+    const int lo = cu[i], hi = cu[i + 1];
+    ok &= lo >= 0 && hi >= lo && (i + 1 < n_seqs || hi <= total);
+  }
+  return ok;
 }
 
 // Launch a kernel; a small grid may start while its predecessor in the stream ends (the kernel calls pdl_wait_prior

@@ -76,6 +76,8 @@ __device__ __forceinline__ void find_leads(const ms_kv4_cache& c, const ms_kv4_r
       ls.tok[k] = tok;
     }
     if (lane == 0) ls.n = __popc(mask);
+  } else if (threadIdx.x < 64) {           // the second warps of all blocks look the offsets over together
+    if (!offsets_ok(r.cu, c.n_seqs, r.total, blockIdx.x * 32, gridDim.x * 32)) atomicOr(err, EF_BAD_INDEX);
   }
   __syncthreads();
 }

@@ -220,7 +220,13 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
   __syncthreads();
   if (CL == 2) cluster_sync();
   umma::fence_after_sync();
+  // the first blocks' (of a pair) last warps, which copy and multiply nothing, look the offsets over together
+  auto look_over = [&]() {
+    const int at = index * 32, step = gridDim.x / CL * 32;
+    if (!offsets_ok(a.cu_q, a.n_seqs, a.total_q, at, step) || !offsets_ok(a.cu_k, a.n_seqs, a.total_k, at, step)) atomicOr(err, EF_BAD_INDEX);
+  };
   if (!pl.ok) {                            // all threads, in both blocks of a pair
+    if (warp == S::SOFTMAX_WARPS + 3 && rank == 0) look_over();
     if (warp == S::SOFTMAX_WARPS) umma::dealloc_cg<CL>(tmem_base, S::COLS);
     return;
   }
@@ -293,6 +299,8 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
         if (role == 3 && clear_tail(j)) fence_cluster();
         if (lane == 0) arrive_at_first(role == 0 ? &k_other[j % ST] : &v_other[j % ST]);
       }
+    } else if (role == 3) {
+      look_over();
     } else if (role == 0) {
       // ---- MMA: the whole warp walks, one thread issues ----
       constexpr uint32_t id_s = umma::idesc_f16(128 * CL, BN, BF16, false), id_o = umma::idesc_f16(128 * CL, HD, BF16, true);

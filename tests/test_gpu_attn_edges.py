@@ -60,3 +60,77 @@ def test_kv4_attention_reports_every_bad_page_number(ctx, page, entry):
     assert e.value.status == 11
     want, A = R.attention(q[0], k[keep], v[keep], torch.tensor([4 * page], device="cuda"), 0, 0.125, None)
     G.within(out[0], want, 2.0 ** -8 * want.abs() + 2.0 ** -8 * A)
+
+
+# ---------------------------------------------------------------- offsets that are not the offsets of packed sequences
+
+def reported(ctx):
+    from moe_stream_b200._lib import MsError
+    with pytest.raises(MsError) as e:
+        ctx.sync()
+    assert e.value.status == 11
+    ctx.sync()
+
+
+def bad_offsets(n, total, how):
+    """Offsets of n sequences of `total` rows, bad in one place."""
+    cu = [i * total // n for i in range(n + 1)]
+    if how == "descends":
+        cu[n // 2] = cu[n // 2 + 1] + 3
+    elif how == "negative":
+        cu[0] = -2
+    elif how == "behind":
+        cu[n] = total + 1
+    else:                                                        # a sequence in the middle begins before its predecessor
+        cu[n // 2 + 1] = max(0, cu[n // 2] - 5)
+    return cu
+
+
+@pytest.mark.parametrize("n", [2, 40, 3000])
+@pytest.mark.parametrize("how", ["descends", "negative", "behind", "overlaps"])
+def test_kv4_rows_report_bad_offsets(ctx, n, how):
+    total = 2 * n + 10
+    cache, raw, table = G.new_cache([32] * n, 16, 1, 64, seed=n)
+    cu, start = G.i32(bad_offsets(n, total, how)), G.i32([0] * n)
+    k = torch.randn(total, 1, 64, device="cuda", generator=G.gen(1)).half()
+    ctx.kv4_write(cache, k, k, cu, start)
+    reported(ctx)
+    nobody = sorted(set(range(raw.shape[0])) - set(table.reshape(-1).tolist()))
+    assert np.array_equal(cache.pages.cpu().numpy()[nobody], raw[nobody])
+    ctx.kv4_read(cache, cu, start, torch.empty_like(k), torch.empty_like(k))
+    reported(ctx)
+    good = G.i32([i * total // n for i in range(n + 1)])
+    ctx.kv4_write(cache, k, k, good, start)
+    ctx.kv4_read(cache, good, start, torch.empty_like(k), torch.empty_like(k))
+    ctx.sync()
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("n", [2, 40, 3000])
+@pytest.mark.parametrize("how", ["descends", "negative", "behind", "overlaps"])
+def test_prompt_attention_reports_bad_offsets(ctx, n, how, hd):
+    total = 2 * n + 10
+    q = torch.randn(total, 4, hd, device="cuda", generator=G.gen(2)).half()
+    k = torch.randn(total, 2, hd, device="cuda", generator=G.gen(3)).half()
+    good, bad, out = G.i32([i * total // n for i in range(n + 1)]), G.i32(bad_offsets(n, total, how)), torch.empty_like(q)
+    for cq, ck in ((bad, good), (good, bad)):
+        ctx.prompt_attention(q, k, k, cq, ck, out)
+        reported(ctx)
+    ctx.prompt_attention(q, k, k, good, good, out)
+    ctx.sync()
+
+
+def test_rows_in_front_of_the_first_sequence_are_left(ctx):
+    """Offsets that begin behind 0 are no error: the rows in front of them are nobody's."""
+    cache, raw, table = G.new_cache([20], 16, 2, 64, seed=1)
+    k = torch.randn(30, 2, 64, device="cuda", generator=G.gen(1)).half()
+    ctx.kv4_write(cache, k, k, G.i32([10, 30]), G.i32([0]))
+    back = torch.full_like(k, 7.0)
+    ctx.kv4_read(cache, G.i32([10, 30]), G.i32([0]), back, torch.empty_like(k))
+    q = torch.randn(30, 4, 64, device="cuda", generator=G.gen(2)).half()
+    out, want = torch.full_like(q, 7.0), torch.empty_like(q[10:])
+    ctx.prompt_attention(q, k, k, G.i32([10, 30]), G.i32([10, 30]), out)
+    ctx.prompt_attention(q[10:], k[10:], k[10:], G.i32([0, 20]), G.i32([0, 20]), want)
+    ctx.sync()
+    assert (back[:10] == 7.0).all() and (back[10:] != 7.0).any()
+    assert (out[:10] == 7.0).all() and torch.equal(out[10:], want)
