@@ -335,7 +335,8 @@ MS_API ms_status ms_kv4_read(ms_ctx* ctx, const ms_kv4_cache* cache, const ms_kv
  * attends tokens j <= that, j > that - window when window > 0; sinks [heads] or NULL.  A query without
  * tokens (lens[i] = 0) gives zeros.  q / out [n_seqs][n_query][heads][head_dim], contiguous, f16 or bf16;
  * scores from the exact codes in f32, probabilities and dequantised V rounded to f16 for the second
- * product (f32 accumulation; with f16 outputs the probabilities' rests are added).  heads a multiple of
+ * product (f32 accumulation; with f16 outputs the probabilities' rests are added; besides its rounding a probability
+ * may be off by 2^-32 of the row's largest).  heads a multiple of
  * kv_heads; n_query * heads / kv_heads <= 128; n_seqs <= 65535.
  * work: ms_kv4_attention_workspace bytes (16-byte aligned) that this call alone uses while it runs: calls
  * (or captured graphs) that may overlap need one each. */

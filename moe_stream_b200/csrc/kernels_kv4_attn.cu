@@ -21,9 +21,11 @@
 // The first part is one more product of the stored (d, o) pairs with R and Q, each cut into two f16 (22 bits);
 // the second is one f32 multiply-add a group.  Values: v = fma(16 + c, d, o) in f16 pairs of two keys, the probabilities in f16 (bf16 would
 // cost 8 times their rounding; with f16 outputs, where it shows, their rests in a second product) transposed by
-// movmatrix from the score layout.  The running maximum is raised
-// only when the probabilities of a tile grow beyond 2^8: p stays far inside f16, and most tiles need no
-// reduction over the lanes.
+// movmatrix from the score layout.  The probabilities are taken against the running maximum less kBelow (7): the largest is
+// 2^7, so those that f16 rounds to a multiple of 2^-24 lie below 2^-21 of it and are off by 2^-32 of it at most (against the
+// maximum itself, keys below 2^-25 of it would have counted in the sum and not in the output: 4,000 keys at 2^-25.5 behind
+// one of 1 lost all of their share).  The maximum is raised only when a lane's probabilities of a tile add up to more than
+// 2^15, 2^8 times the largest: p stays inside f16, and most tiles need no reduction over the lanes.
 //
 // Measured: 32 sequences of 8,300 tokens on average, 4 heads of 128 dims (162 MB): 43 us, 3.7 TB/s; one of 131,072
 // tokens, 8 heads of 64 dims (84 MB, f16): 28 us; one of 4,097 tokens: 9 us.  Bulk copies alone stream the first
@@ -52,7 +54,8 @@ constexpr int kMinTiles = kWarps;         // tiles of a range at least: one per 
 constexpr int kExtra = 8;                 // empty tiles behind those of a job
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;           // the running maximum before any key
-constexpr float kRaise = 256.0f;          // sum of a lane's probabilities of a tile that raises the maximum
+constexpr float kBelow = 7.0f;            // powers of two that the probabilities' base lies below the maximum
+constexpr float kRaise = 32768.0f;        // sum of a lane's probabilities of a tile that raises the maximum
 
 // ---- the list of tiles ----
 struct Plan {        // (the callers check that all tiles of a cache's capacity are below 2^31)
@@ -226,7 +229,7 @@ struct Rows {
   uint32_t corr[NT][CORR][2];
   float c2[NT][2];         // log2(e) scale times the row's power of two
   int last[NT][2];         // the row's last key (-1: no such row)
-  float o[NT][MT][4], m[NT][2], l[NT][2];
+  float o[NT][MT][4], m[NT][2], l[NT][2];   // m: the base of the probabilities, kBelow under the running maximum
 };
 
 // one tile: scores, probabilities, value product.  MASKED: some keys are not every row's
@@ -300,7 +303,7 @@ __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const Bases& K, const
         }
     }
   }
-  // probabilities against the running maximum; when they grow too large it is raised first
+  // probabilities against the running base; when they grow too large it is raised first
   float p[TB][NT][4];
   auto exps = [&]() {
     bool far = false;
@@ -333,7 +336,7 @@ __device__ __forceinline__ void take_tile(Rows<HD, NT>& R, const Bases& K, const
         for (int b = 0; b < TB; ++b) top = fmaxf(top, fmaxf(s[b][n][i], s[b][n][2 + i]));
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        top = fmaxf(top * R.c2[n][i], R.m[n][i]);
+        top = fmaxf(fmaf(top, R.c2[n][i], -kBelow), R.m[n][i]);
         const float f = exp2_fast(R.m[n][i] - top);
         R.m[n][i] = top;
         R.l[n][i] = l0[n][i] * f;

@@ -134,3 +134,46 @@ def test_rows_in_front_of_the_first_sequence_are_left(ctx):
     ctx.sync()
     assert (back[:10] == 7.0).all() and (back[10:] != 7.0).any()
     assert (out[:10] == 7.0).all() and torch.equal(out[10:], want)
+
+
+# ---------------------------------------------------------------- one large score in front of many small ones
+
+def spike_rows(n, hd, seed):
+    """K and V rows of one kv head: key 0 is all ones with v = 0, the others are zeros with v between 1 and 1.25."""
+    g = G.gen(seed)
+    k = torch.zeros(n, 1, hd, device="cuda")
+    k[0] = 1.0
+    v = 1 + 0.25 * torch.rand(n, 1, hd, device="cuda", generator=g)
+    v[0] = 0
+    return k, v
+
+
+def spike_queries(n, hd, drop, t):
+    """One query of n heads: the probability of key 0 is 2^drop[head] times that of any other key."""
+    q = torch.tensor(drop, device="cuda")[None, :, None] / (np.log2(np.e) * hd ** 0.5)
+    return q.expand(1, n, hd).contiguous().to(t)
+
+
+DROPS = [0.0, 14.5, 20.5, 24.9, 25.5, 26.0, 27.5, 29.0]            # 2^-25 and below round to 0 in f16
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("t", ["float16", "bfloat16"])
+def test_kv4_attention_large_score_and_flat_tail(ctx, hd, t):
+    """All that the output has comes from keys with probabilities of 2^-14.5 .. 2^-29 of the largest.  512 sequences that
+    share one's pages, so that a warp takes many keys behind the large one.  Besides the roundings of G.cached_reference, a
+    probability is off by half an f16 subnormal, 2^-25 where the largest is 2^7 or more: 2^-32 of it for each key."""
+    from moe_stream_b200.engine import KV4Cache
+    t, n, seqs = getattr(torch, t), 4000, 512
+    one, _, table = G.new_cache([n], 16, 1, hd, seed=1)
+    k, v = spike_rows(n, hd, 2)
+    ctx.kv4_write(one, k, v, G.i32([0, n]), G.i32([0]))
+    ctx.sync()
+    cache = KV4Cache(one.pages, one.block_table.expand(seqs, -1).contiguous(), 1, hd, 16)
+    q = spike_queries(len(DROPS), hd, DROPS, t)[None].expand(seqs, -1, -1, -1).contiguous()
+    out = torch.empty_like(q)
+    work = torch.empty(ctx.kv4_attention_workspace_bytes(cache, seqs, 1, len(DROPS)), dtype=torch.uint8, device="cuda")
+    ctx.kv4_attention(cache, q, G.i32([n] * seqs), out, work)
+    ctx.sync()
+    want, tol = G.cached_reference(one, table, q[:1], [n], 0, hd ** -0.5, None)
+    G.within(out, want.expand_as(out), (tol + n * 2.0 ** -32 * 1.25).expand_as(out))
