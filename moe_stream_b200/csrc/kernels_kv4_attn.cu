@@ -437,16 +437,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
   Cursor cur = find_tile<TT>(c, a, plan, u0), pre = cur;
   // ---- the ring: tiles warp, warp + kWarps, ... of the range; `page` is looked up one tile ahead ----
   const bool one_page = (1 << shift) >= TT;                  // a tile lies inside one page (else lane p brings page p of it)
+  int page = 0;
+  bool want = false;                                         // the lane brings that page (nothing looks at it before the copy)
   auto look_up = [&]() {
     const int token = (pre.s.first + pre.tile) * TT + (one_page ? 0 : lane << shift);
-    const bool want = lane < (one_page ? 1 : TT >> shift) && token < pre.s.len && token + c.page_tokens > pre.s.lo;
-    return want ? max(c.block_table[(int64_t)pre.seq * c.max_pages + (token >> shift)], -1) : -2;   // -2: not needed
+    want = lane < (one_page ? 1 : TT >> shift) && token < pre.s.len && token + c.page_tokens > pre.s.lo;
+    if (want) page = c.block_table[(int64_t)pre.seq * c.max_pages + (token >> shift)];
   };
-  auto fetch = [&](int k, int page) {                        // the warp's tile number k
+  auto fetch = [&](int k) {                                  // the warp's tile number k
     const int stage = k % kStages;
     const int head = row_tiles > 1 ? pre.job / row_tiles : pre.job;
-    const bool ok = (unsigned)page < (unsigned)c.n_pages;
-    if (page != -2 && !ok) atomicOr(err, EF_BAD_INDEX);
+    const bool ok = want && (unsigned)page < (unsigned)c.n_pages;
+    if (want && !ok) atomicOr(err, EF_BAD_INDEX);
     const int n_blk = one_page ? TB : 1 << (shift - 4);      // blocks that a lane copies
     uint32_t have = ok ? ((1u << n_blk) - 1) << (one_page ? 0 : lane * n_blk) : 0u;
     if (!one_page) have = __reduce_or_sync(0xffffffffu, have);
@@ -462,16 +464,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
       bulk_g2s(sm.stage[warp][stage] + lane * n_blk * BLK, (const uint8_t*)c.pages + blk * BLK, n_blk * BLK, &sm.full[warp][stage]);
     }
   };
-  int next = warp, used = 0, page = -2;                      // next tile to fetch; tiles taken by this warp
+  int next = warp, used = 0;                                 // next tile to fetch; tiles taken by this warp
   auto step_next = [&](int n) {                              // to the warp's next tile that is not empty
     do {
       advance<TT>(c, a, plan.jobs, pre, n);
       n = kWarps;
     } while (next < count && pre.tile >= pre.s.n && (next += kWarps) < count);
-    if (next < count) page = look_up();
+    if (next < count) look_up();
   };
   auto fetch_next = [&](int k) {
-    fetch(k, page);
+    fetch(k);
     next += kWarps;
     step_next(kWarps);
   };
