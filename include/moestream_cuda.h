@@ -277,7 +277,8 @@ MS_API ms_status ms_qk_norm_rope(ms_ctx* ctx, const ms_qk_rope* args);
  * with more keys than queries continues a cached prefix.  Query at key index p attends keys j <= p, and
  * j > p - window when window > 0; sinks [heads] (f32, or NULL) join the softmax denominator.
  * out = softmax(scale q k^T) v in f32 with the probabilities rounded to the element type for the second
- * product; a query without keys gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.
+ * product (f16: besides that rounding a probability may be off by 2^-32 of the row's largest); a query without keys
+ * gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.
  * total_q / total_k: rows of q and out / of k and v (cu_q[n_seqs] and cu_k[n_seqs] at most).  Offsets that descend, are
  * negative or end behind these are reported (MS_ERR_DEVICE_INDEX); out then holds nothing of use for any sequence.
  * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 128 per kv head and 65536; strides multiples of

@@ -14,8 +14,11 @@
 // the scores, writes the probabilities as 16-bit pairs, and the value product takes them from tensor memory.  With
 // 128 and 256 dims they lie over the scores they came from, which the MMA warp overwrites next: the MMAs of
 // one thread execute in the order of issue.  The running maximum is that of the row's first tile until the
-// probabilities of a later one add up to more than kRaise: only then the tile's maximum is looked for and the output
-// rescaled, and no probability comes near the largest f16.  Sums are in f32 over the unrounded probabilities.
+// probabilities of a later one add up to too much (Range): only then the tile's maximum is looked for and the output
+// rescaled, and no probability comes beyond the largest f16.  In f16 the probabilities are taken against the maximum less
+// 7, so the largest is 2^7 and those that f16 rounds to a multiple of 2^-24 are off by 2^-32 of it at most (against the maximum
+// itself, keys below 2^-25 of it would have counted in the sum and not in the output).  Sums are in f32 over the unrounded
+// probabilities.
 //
 // Values of keys behind the sequence's end (other rows of the packed buffer, perhaps not finite) are zeroed in
 // shared memory before the last product; their scores are masked.
@@ -46,7 +49,16 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -1e30f;   // the running maximum before any key
-constexpr float kRaise = 4096.f;  // sum of a row's probabilities of a tile that raises the running maximum
+// powers of two that the probabilities' base lies below the running maximum, and the sum of a row's probabilities of a
+// tile that raises it (f16: its largest number; bf16 has the range of f32)
+template <class T>
+struct Range {
+  static constexpr float below = 0.f, raise = 4096.f;
+};
+template <>
+struct Range<__half> {
+  static constexpr float below = 7.f, raise = 65504.f;
+};
 
 // CL: blocks that share an MMA (a pair reads each K and V tile once for twice the rows, half of it each)
 template <int HD, int CL>
@@ -449,7 +461,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
           for (int i = 8; i < BN; i += 8)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top4[e] = max3(top4[e], __uint_as_float(u[i + 2 * e]), __uint_as_float(u[i + 2 * e + 1]));
-          const float top = fmaxf(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c2, m), f = exp2_fast(m - top);
+          const float top = fmaxf(fmaf(fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])), c2, -Range<T>::below), m), f = exp2_fast(m - top);
           m = top;
           l *= f;
           return f;
@@ -471,7 +483,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
         load();
         if (j == 0) raise_max();
         float sum = exps();
-        if (__any_sync(0xffffffffu, sum > kRaise)) {         // (not with the first tile, whose maximum was taken)
+        if (__any_sync(0xffffffffu, sum > Range<T>::raise)) {         // (not with the first tile, whose maximum was taken)
           load();
           const float f = raise_max();
           sum = exps();

@@ -177,3 +177,19 @@ def test_kv4_attention_large_score_and_flat_tail(ctx, hd, t):
     ctx.sync()
     want, tol = G.cached_reference(one, table, q[:1], [n], 0, hd ** -0.5, None)
     G.within(out, want.expand_as(out), (tol + n * 2.0 ** -32 * 1.25).expand_as(out))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("t", ["float16", "bfloat16"])
+def test_prompt_attention_large_score_and_flat_tail(ctx, hd, t):
+    """The same for one query behind 4,000 keys (each head a drop): f16 probabilities are off by 2^-32 of the largest for
+    each key, bf16 ones by nothing besides their rounding."""
+    t, n, H = getattr(torch, t), 4000, len(DROPS)
+    k, v = (x.to(t) for x in spike_rows(n, hd, 3))
+    q = spike_queries(H, hd, DROPS, t)
+    out = torch.empty_like(q)
+    cq, ck = G.i32([0, 1]), G.i32([0, n])
+    ctx.prompt_attention(q, k, v, cq, ck, out)
+    ctx.sync()
+    want, tol = G.prompt_reference(q, k, v, [1], [n], 0, hd ** -0.5, None)
+    G.within(out, want, tol + n * 2.0 ** -32 * 1.25)
