@@ -275,7 +275,7 @@ MS_API ms_status ms_qk_norm_rope(ms_ctx* ctx, const ms_qk_rope* args);
 /* Causal attention of n_seqs packed sequences: queries cu_q[i] .. cu_q[i + 1] (rows of q and out) over
  * keys cu_k[i] .. cu_k[i + 1] (rows of k and v); the last query stands at the last key, so a sequence
  * with more keys than queries continues a cached prefix.  Query at key index p attends keys j <= p, and
- * j > p - window when window > 0; sinks [heads] (f32, or NULL) join the softmax denominator.
+ * j > p - window when window > 0; sinks [heads] (f32, or NULL; infinite ones too) join the softmax denominator.
  * out = softmax(scale q k^T) v in f32 with the probabilities rounded to the element type for the second
  * product (f16: besides that rounding a probability may be off by 2^-32 of the row's largest); a query without keys
  * gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.

@@ -118,6 +118,14 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return r;
 }
 
+// A sink's share of a softmax denominator on base `top`, both as powers of two and top >= sink unless sink is NaN.  An
+// infinite sink is its own base (everything else counts 0 on it); a NaN stays one.
+__device__ __forceinline__ float sink_share(float sink, float top) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(sink == top ? 0.f : sink - top));
+  return r;
+}
+
 // One warp's share, 32 of every `step` sequences from `first` on, of the check of offsets cu [n_seqs + 1]: false in a lane
 // that sees a negative or descending one, or an end behind `total`.
 __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int n_seqs, int total, int first, int step) {

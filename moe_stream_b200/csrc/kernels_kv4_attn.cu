@@ -650,12 +650,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(HD, NT)) kv4_attn_kern
       if (done) {
         const int h = head * rep + rr % rep;
         float f = 1.f;
-        if (a.sinks) {
+        if (a.sinks && sum != 0.f) {
           const float sink = a.sinks[h] * kLog2e, base = fmaxf(top, sink);
           f = exp2_fast(top - base);
-          sum = sum * f + exp2_fast(sink - base);
+          sum = sum * f + sink_share(sink, base);
         }
-        f = sum > 0.f ? f / sum : 0.f;
+        f = sum == 0.f ? 0.f : f / sum;                      // (no keys: zeros)
         T* dst = (T*)a.out + (((int64_t)cur.seq * a.n_query + rr / rep) * a.heads + h) * HD + d;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
       } else {
@@ -733,7 +733,8 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const ms_kv4_cache c
   float top = sink;
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, ms[i]);
-  l = a.sinks ? exp2_fast(sink - top) : 0.f;
+  l = a.sinks ? sink_share(sink, top) : 0.f;
+  float keys = 0.f;                        // 0: the row has none
   v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i) {
@@ -741,8 +742,9 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(const ms_kv4_cache c
     const float f = exp2_fast(ms[i] - top);
     v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
     l += f * ls[i];
+    keys += ls[i];
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = keys == 0.f ? 0.f : 1.f / l;
   T* dst = (T*)a.out + (((int64_t)seq * a.n_query + rr / rep) * a.heads + h) * HD + 4 * col;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
 }

@@ -527,11 +527,11 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
         float den = l;
         f = 1.f;
         if (a.sinks) {
-          const float sink = a.sinks[h < a.heads ? h : 0] * kLog2e, mm = fmaxf(m, sink);
+          const float sink = a.sinks[h] * kLog2e, mm = fmaxf(m, sink);
           f = exp2_fast(m - mm);
-          den = l * f + exp2_fast(sink - mm);
+          den = l * f + sink_share(sink, mm);
         }
-        f = den > 0.f ? f / den : 0.f;       // (an infinite sink takes everything)
+        f /= den;
       }
       T* dst = (T*)a.out + (int64_t)(pl.q0 + tok) * a.out_stride + h * HD;
 #pragma unroll

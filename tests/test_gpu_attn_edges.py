@@ -193,3 +193,31 @@ def test_prompt_attention_large_score_and_flat_tail(ctx, hd, t):
     ctx.sync()
     want, tol = G.prompt_reference(q, k, v, [1], [n], 0, hd ** -0.5, None)
     G.within(out, want, tol + n * 2.0 ** -32 * 1.25)
+
+
+# ---------------------------------------------------------------- sinks that are no numbers
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("longest", [40, 9000])                      # one block's part of a job, and joined parts
+def test_a_nan_sink_reaches_its_head_alone(ctx, hd, longest):
+    """A NaN sink makes its head's rows NaN, where they have keys; the other heads, with finite and infinite sinks, are as
+    without it."""
+    H = 8
+    case = ([longest, 0, 3], 4, 16, H, 2, hd, 0, False, "float16")
+    cache, table, q, lens, out, work, _, _ = G.cached_case(ctx, case, poison=True)
+    pq, pk, pv, cq, ck, _, _ = G.prompt_case([70, 40], [0, 9], H, 2, hd, torch.float16)
+    sk = torch.randn(H, device="cuda", generator=G.gen(9))
+    sk[1], sk[6] = float("inf"), float("-inf")
+    bad = sk.clone()
+    bad[3] = float("nan")
+    nan, pn, pw = torch.empty_like(out), torch.empty_like(pq), torch.empty_like(pq)
+    ctx.kv4_attention(cache, q, lens, out, work, sinks=sk)
+    ctx.kv4_attention(cache, q, lens, nan, work, sinks=bad)
+    ctx.prompt_attention(pq, pk, pv, cq, ck, pw, sinks=sk)
+    ctx.prompt_attention(pq, pk, pv, cq, ck, pn, sinks=bad)
+    ctx.sync()
+    keep = [h for h in range(H) if h != 3]
+    assert torch.equal(nan[:, :, keep], out[:, :, keep]) and torch.equal(pn[:110, keep], pw[:110, keep])
+    assert torch.isnan(nan[0, :, 3]).all() and torch.isnan(nan[2, 1:, 3]).all() and torch.isnan(pn[:110, 3]).all()
+    assert (nan[1, :, 3] == 0).all() and (nan[2, 0, 3] == 0).all()   # queries without keys
+    assert (out[:, :, 1] == 0).all() and (pw[:110, 1] == 0).all()
