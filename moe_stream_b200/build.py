@@ -1,7 +1,9 @@
 """Build libmoestream_cuda (shared, for ctypes / FFI callers, and static, for a Rust build.rs)
-in-tree under moe_stream_b200/_build/ with nvcc for sm_100a, and the extension that reads torch tensors.  Run: python -m moe_stream_b200.build"""
+in-tree under moe_stream_b200/_build/ with nvcc for sm_100a, and, where torch is installed, the extension that reads
+torch tensors.  Run: python -m moe_stream_b200.build"""
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
@@ -39,9 +41,11 @@ def build(verbose: bool = False) -> str:
             cmds.append([NVCC, *FLAGS, "-c", s, "-o", o])
         objs.append(o)
     src = os.path.join(CSRC, "binding.cpp")
-    if _stale(BINDING, [src, headers[-1]]):
-        import torch
-        at = os.path.dirname(torch.__file__)
+    torch = importlib.util.find_spec("torch")                # found, not imported: the library itself needs none
+    if torch is None:
+        print("torch is not installed: the library is built without the extension for torch tensors", file=sys.stderr)
+    elif _stale(BINDING, [src, headers[-1]]):
+        at = os.path.dirname(torch.origin)
         cmds.append(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-isystem", os.path.join(at, "include"),
                      "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING, "-L" + os.path.join(at, "lib"), "-lc10",
                      "-ltorch_cpu", "-ltorch_python"])
