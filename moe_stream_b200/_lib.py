@@ -14,6 +14,7 @@ import re
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_build", "libmoestream_cuda.so")
 BINDING_PATH = os.path.join(HERE, "_build", "_binding.so")
+BINDING_TORCH = os.path.join(HERE, "_build", "_binding.torch")   # the version.py of the torch it was compiled against
 HEADER = os.path.join(os.path.dirname(HERE), "include", "moestream_cuda.h")
 
 MS_OK = 0
@@ -220,7 +221,11 @@ def binding():
     if _binding is None:
         if not os.path.exists(BINDING_PATH):
             raise OSError(f"{BINDING_PATH} is missing: build it with `python -m moe_stream_b200.build`")
-        import torch  # noqa: F401  (loads the libraries that the extension needs)
+        import torch  # (loads the libraries that the extension needs)
+        if os.path.exists(BINDING_TORCH):
+            with open(os.path.join(os.path.dirname(torch.__file__), "version.py")) as now, open(BINDING_TORCH) as then:
+                if now.read() != then.read():
+                    raise OSError(f"{BINDING_PATH} was compiled against another torch: build it with `python -m moe_stream_b200.build`")
         loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
         m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
         loader.exec_module(m)

@@ -20,6 +20,7 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std
 SO = os.path.join(OUT, "libmoestream_cuda.so")
 A = os.path.join(OUT, "libmoestream_cuda.a")
 BINDING = os.path.join(OUT, "_binding.so")
+BINDING_TORCH = os.path.join(OUT, "_binding.torch")   # version.py of the torch that the extension was compiled against
 
 
 def _stale(target: str, deps) -> bool:
@@ -27,6 +28,13 @@ def _stale(target: str, deps) -> bool:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _text(path: str) -> str:
+    if not os.path.exists(path):
+        return ""
+    with open(path) as f:
+        return f.read()
 
 
 def build(verbose: bool = False) -> str:
@@ -41,14 +49,19 @@ def build(verbose: bool = False) -> str:
             cmds.append([NVCC, *FLAGS, "-c", s, "-o", o])
         objs.append(o)
     src = os.path.join(CSRC, "binding.cpp")
-    torch = importlib.util.find_spec("torch")                # found, not imported: the library itself needs none
+    torch, version = importlib.util.find_spec("torch"), None   # found, not imported: the library itself needs none
     if torch is None:
         print("torch is not installed: the library is built without the extension for torch tensors", file=sys.stderr)
-    elif _stale(BINDING, [src, headers[-1]]):
+    else:
         at = os.path.dirname(torch.origin)
-        cmds.append(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-isystem", os.path.join(at, "include"),
-                     "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING, "-L" + os.path.join(at, "lib"), "-lc10",
-                     "-ltorch_cpu", "-ltorch_python"])
+        version = _text(os.path.join(at, "version.py"))
+        if _stale(BINDING, [src, headers[-1]]) or _text(BINDING_TORCH) != version:
+            for old in (BINDING, BINDING_TORCH):
+                if os.path.exists(old):
+                    os.remove(old)
+            cmds.append(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-isystem", os.path.join(at, "include"),
+                         "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING, "-L" + os.path.join(at, "lib"), "-lc10",
+                         "-ltorch_cpu", "-ltorch_python"])
     # translation units compile in parallel (one compiler process each)
     procs = []
     for cmd in cmds:
@@ -58,6 +71,9 @@ def build(verbose: bool = False) -> str:
     failed = [cmd for cmd, p in procs if p.wait() != 0]
     if failed:
         raise subprocess.CalledProcessError(1, failed[0])
+    if version is not None and _text(BINDING_TORCH) != version:
+        with open(BINDING_TORCH, "w") as f:
+            f.write(version)
     if _stale(SO, objs):
         subprocess.run([NVCC, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", SO, *objs,
                         "-Xcompiler", "-fPIC", "-lcuda"], check=True)

@@ -44,3 +44,31 @@ def test_the_library_builds_without_torch(tree):
     assert {"libmoestream_cuda.so", "libmoestream_cuda.a", "runtime.o"} <= set(made)
     assert "_binding.so" not in made and "torch is not installed" in said
     assert (tree / "moe_stream_b200" / "_build" / "libmoestream_cuda.a").exists()
+
+
+def test_the_extension_is_built_again_for_another_torch(tree):
+    at = tree / "site" / "torch"
+    at.mkdir(parents=True)
+    (at / "__init__.py").write_text("raise ImportError('the build imports no torch')")
+    (at / "version.py").write_text("__version__ = '1'")
+    assert "_binding.so" in run(tree, [tree / "site"])[0]
+    assert run(tree, [tree / "site"])[0] == []                       # nothing is stale
+    os.utime(at / "version.py", (0, 0))                              # older files, another version
+    (at / "version.py").write_text("__version__ = '2'")
+    os.utime(at / "version.py", (0, 0))
+    assert run(tree, [tree / "site"])[0] == ["_binding.so"]
+
+
+def test_an_extension_for_another_torch_is_not_loaded(monkeypatch, tmp_path):
+    pytest.importorskip("torch")
+    from moe_stream_b200 import _lib
+    so, stamp = tmp_path / "_binding.so", tmp_path / "_binding.torch"
+    monkeypatch.setattr(_lib, "BINDING_PATH", str(so))
+    monkeypatch.setattr(_lib, "BINDING_TORCH", str(stamp))
+    monkeypatch.setattr(_lib, "_binding", None)
+    with pytest.raises(OSError, match="missing"):
+        _lib.binding()
+    so.write_text("")
+    stamp.write_text("__version__ = '0'")
+    with pytest.raises(OSError, match="another torch"):
+        _lib.binding()
