@@ -56,6 +56,11 @@ float number(PyObject* o) {
   if (v == -1.0 && PyErr_Occurred()) throw PythonError();
   return (float)v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PythonError();
+  return v == 1;
+}
 void* pointer(PyObject* o) {
   if (o == Py_None) return nullptr;
   void* p = PyLong_AsVoidPtr(o);
@@ -149,7 +154,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t n = q.size(0), heads = q.size(1), hd = q.size(2), kv = k.size(1), table = cos.size(0), half = cos.size(1);
     ms_qk_rope r = {};
     r.n_tokens = as_int("the tokens", n); r.heads = as_int("the heads", heads); r.kv_heads = as_int("the heads", kv);
-    r.head_dim = as_int("head_dim", hd); r.rot_dim = as_int("the rotated dims", 2 * half); r.interleaved = PyObject_IsTrue(a[12]) == 1;
+    r.head_dim = as_int("head_dim", hd); r.rot_dim = as_int("the rotated dims", 2 * half); r.interleaved = truth(a[12]);
     r.in_type = type_id(q); r.out_type = type_id(q_out);
     r.eps = number(a[6]);
     r.max_pos = as_int("the positions", table);

@@ -237,3 +237,11 @@ def test_binding_takes_strided_rows_and_one_token(calls):
         with pytest.raises(_lib.MsError) as e:
             calls.call("qk_norm_rope", **change)
         assert e.value.status == INVALID
+
+
+def test_binding_refuses_what_is_neither_true_nor_false(calls):
+    class Neither:
+        def __bool__(self):
+            raise RuntimeError("neither")
+    with pytest.raises(RuntimeError, match="neither"):
+        calls.call("qk_norm_rope", interleaved=Neither())
