@@ -142,7 +142,7 @@ __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int n_seqs, int to
 // grid would only take room from the predecessor: a cache write and read of 8,900 tokens took 19.0 us so, 17.0 without.
 // The error is left to cudaGetLastError.
 template <class... P, class... A>
-inline void launch_early(void (*kernel)(P...), uint32_t grid, uint32_t threads, cudaStream_t s, A... args) {
+inline void launch_early(void (*kernel)(P...), int sm_count, uint32_t grid, uint32_t threads, cudaStream_t s, A... args) {
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -151,7 +151,7 @@ inline void launch_early(void (*kernel)(P...), uint32_t grid, uint32_t threads, 
   cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cfg.attrs = at;
-  cfg.numAttrs = grid <= 296 ? 1 : 0;
+  cfg.numAttrs = grid <= 2u * sm_count ? 1 : 0;   // two blocks an SM at most
   cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 

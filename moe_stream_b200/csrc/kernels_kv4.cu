@@ -330,8 +330,8 @@ cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_rows& r, 
   int rows = kRows;
   while (rows > 2 && (int64_t)r.total < (int64_t)rows * 4 * d.sm_count) rows /= 2;
   const uint32_t grid = (uint32_t)(((int64_t)r.total + rows - 1) / rows);
-  if (write) launch_early(kv4_write_kernel<T, HD>, grid, kThreads, s, c, r, rows, d.err);
-  else launch_early(kv4_read_kernel<T, HD>, grid, kThreads, s, c, r, rows, d.err);
+  if (write) launch_early(kv4_write_kernel<T, HD>, d.sm_count, grid, kThreads, s, c, r, rows, d.err);
+  else launch_early(kv4_read_kernel<T, HD>, d.sm_count, grid, kThreads, s, c, r, rows, d.err);
   return cudaGetLastError();
 }
 

@@ -63,9 +63,10 @@ struct Range<__half> {
 // CL: blocks that share an MMA (a pair reads each K and V tile once for twice the rows, half of it each)
 template <int HD, int CL>
 struct Shape {
-  static constexpr int NQ = HD == 256 ? 1 : 2;          // query tiles of a block
+  static_assert(CL == (HD == 256 ? 2 : 1));             // pairs of blocks have one query tile each
+  static constexpr int NQ = CL == 2 ? 1 : 2;            // query tiles of a block
   static constexpr int BN = 128;                        // keys of a tile
-  static constexpr int STAGES = HD == 64 ? 4 : 2 * (HD == 256 ? 1 : CL);   // of K and of V
+  static constexpr int STAGES = HD == 64 ? 4 : 2;       // of K and of V
   static constexpr int Q_BYTES = 128 * HD * 2, KV_BYTES = BN * HD * 2 / CL;
   static constexpr int K_ROWS = BN / CL, V_BLOCKS = HD / 64 / CL;   // a block's share: rows of K, blocks of 64 dims of V
   static constexpr int SOFTMAX_WARPS = 4 * NQ, THREADS = 32 * (SOFTMAX_WARPS + 4);
@@ -245,8 +246,8 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
   constexpr uint32_t tmem = 0;             // all 512 columns are this block's, so they start at 0
   if (threadIdx.x == 0 && tmem_base != tmem) atomicOr(err, EF_BAD_SHAPE);
   const int nq = pl.q1 - pl.q0, nk = pl.k1 - pl.k0;
-  // query tile i of this block begins at token t0 + (i CL + rank) n_tok; slots: tiles with rows in any of the blocks
-  const int slots = NQ == 2 && pl.t0 + CL * n_tok < nq ? 2 : 1;
+  // query tile i of this block begins at token t0 + (i + rank) n_tok; slots: the block's tiles that have rows
+  const int slots = NQ == 2 && pl.t0 + n_tok < nq ? 2 : 1;
 
   // the two softmax groups need more than the 168 registers of 384 threads: 208 x 256 + 80 x 128 of 168 x 384
   if (warp >= S::SOFTMAX_WARPS) {
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
           mbar_expect_tx(&q_full, slots * BLK * rows * 128);
           for (int i = 0; i < slots; ++i)
             for (int b = 0; b < BLK; ++b)
-              tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + (i * CL + rank) * n_tok, &q_full);
+              tma_3d(sq + i * S::Q_BYTES + b * 128 * 128, &q_map, 64 * b, head * rep, pl.q0 + pl.t0 + (i + rank) * n_tok, &q_full);
         }
         int j = 0;
         for (; j < pl.tiles; ++j) {
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(Shape<HD, CL>::THREADS, 1)
     // ---- softmax: thread = row ----
     if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int tile = warp >> 2, r = threadIdx.x & 127;       // query tile of the block, row of it
-    const int tok = pl.t0 + (tile * CL + rank) * n_tok + r / rep;   // token of the sequence
+    const int tok = pl.t0 + (tile + rank) * n_tok + r / rep;   // token of the sequence
     const bool row_ok = r < n_tok * rep && tok < nq;
     const int h = head * rep + r % rep;
     const int last = row_ok ? nk - nq + tok : -1;            // the row's last key

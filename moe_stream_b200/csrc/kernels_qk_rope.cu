@@ -154,11 +154,11 @@ __global__ void __launch_bounds__(kThreads) qk_rope_any_kernel(const ms_qk_rope 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <class TI, class TO, int LPR, int HPG>
-void start_vec(const ms_qk_rope& a, uint32_t* err, cudaStream_t s) {
+void start_vec(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
   const uint32_t nb = (a.heads + HPG - 1) / HPG + (a.kv_heads + HPG - 1) / HPG;
   const uint32_t grid = ((uint64_t)a.n_tokens * nb + kThreads / LPR - 1) / (kThreads / LPR);
-  if (a.interleaved) launch_early(qk_rope_kernel<TI, TO, LPR, HPG, true>, grid, kThreads, s, a, err);
-  else launch_early(qk_rope_kernel<TI, TO, LPR, HPG, false>, grid, kThreads, s, a, err);
+  if (a.interleaved) launch_early(qk_rope_kernel<TI, TO, LPR, HPG, true>, c.sm_count, grid, kThreads, s, a, c.err);
+  else launch_early(qk_rope_kernel<TI, TO, LPR, HPG, false>, c.sm_count, grid, kThreads, s, a, c.err);
 }
 
 template <class TI, class TO>
@@ -170,16 +170,16 @@ void start(const DevCtx& c, const ms_qk_rope& a, cudaStream_t s) {
                    aligned16(a.q_norm) && aligned16(a.k_norm);
   if (!vec) {
     const uint64_t items = (uint64_t)a.n_tokens * (a.heads + a.kv_heads);
-    launch_early(qk_rope_any_kernel<TI, TO>, (uint32_t)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, s, a, c.err);
+    launch_early(qk_rope_any_kernel<TI, TO>, c.sm_count, (uint32_t)((items + kThreads / 32 - 1) / (kThreads / 32)), kThreads, s, a, c.err);
     return;
   }
   // Four heads per group share a look-up and the table's row; with few rows one, so that the loads spread over the
   // SMs.  32 + 4 heads of 128 dims, four against one: 2.3 / 1.6 us (1 token), 2.5 / 1.8 (32), 2.7 / 2.7 (256),
   // 4.6 / 6.1 (1,024), 12.6 / 17.6 (4,096).
   const bool wide = (int64_t)a.n_tokens * (a.heads + a.kv_heads) * hd / 16 >= (int64_t)c.sm_count * 512;
-  if (hd == 64) wide ? start_vec<TI, TO, 4, 4>(a, c.err, s) : start_vec<TI, TO, 4, 1>(a, c.err, s);
-  else if (hd == 128) wide ? start_vec<TI, TO, 8, 4>(a, c.err, s) : start_vec<TI, TO, 8, 1>(a, c.err, s);
-  else wide ? start_vec<TI, TO, 16, 4>(a, c.err, s) : start_vec<TI, TO, 16, 1>(a, c.err, s);
+  if (hd == 64) wide ? start_vec<TI, TO, 4, 4>(c, a, s) : start_vec<TI, TO, 4, 1>(c, a, s);
+  else if (hd == 128) wide ? start_vec<TI, TO, 8, 4>(c, a, s) : start_vec<TI, TO, 8, 1>(c, a, s);
+  else wide ? start_vec<TI, TO, 16, 4>(c, a, s) : start_vec<TI, TO, 16, 1>(c, a, s);
 }
 
 template <class TI>
