@@ -246,8 +246,9 @@ MS_API ms_status ms_model_batch_profile_step(ms_model* m, float* us, int max, in
  *   - check sizes, strides and types on the host (MS_ERR_INVALID_ARG: a pointer is missing;
  *     MS_ERR_SHAPE: a size, stride or alignment; MS_ERR_UNSUPPORTED_QTYPE: a type) before anything
  *     is launched, also when ctx is NULL (a dry run of the checks that ends in MS_ERR_INVALID_ARG);
- *   - check what only the device knows (positions, lengths, page numbers) in the kernel: a bad entry
- *     is skipped and raises MS_ERR_DEVICE_INDEX at the next ms_sync;
+ *   - check what only the device knows (positions, lengths, offsets, page numbers) in the kernel: a bad
+ *     entry is skipped and raises MS_ERR_DEVICE_INDEX at the next ms_sync (a call without rows launches
+ *     and checks nothing);
  *   - take element types MS_Q_F16 and MS_Q_BF16 (MS_Q_F32 where stated) and strides in elements
  *     between tokens; the heads of one token are contiguous. */
 
@@ -321,7 +322,8 @@ MS_API ms_status ms_kv4_page_bytes(int kv_heads, int head_dim, int page_tokens, 
  * cache back into them (rounded once from f32): rows cu[i] .. cu[i + 1] are the tokens start[i],
  * start[i] + 1, ... of sequence i.  Rows behind cu[n_seqs] are skipped.  Offsets that descend, are negative or end
  * behind `total` are reported (MS_ERR_DEVICE_INDEX); which of the sequences' tokens and rows were taken then is open.
- * Writing touches the bytes of its own tokens only; two calls that write the same token at the same time leave either. */
+ * Writing touches the bytes of its own tokens only; a token that is written twice at the same time (by two calls, or by two
+ * sequences of a call that share a page) holds the codes and scales of both in any mixture. */
 typedef struct ms_kv4_rows {
   int type, total;
   const int32_t *cu, *start;   /* [n_seqs + 1] ascending from 0, [n_seqs] (device) */

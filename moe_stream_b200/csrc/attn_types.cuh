@@ -139,7 +139,7 @@ __device__ __forceinline__ bool offsets_ok(const int32_t* cu, int n_seqs, int to
 
 // Launch a kernel; a small grid may start while its predecessor in the stream ends (the kernel calls pdl_wait_prior
 // before it touches memory), which saves a decode step about a microsecond a kernel.  The waiting blocks of a large
-// grid would only take room from the predecessor: a cache write and read of 8,900 tokens took 19.0 us so, 17.0 without.
+// grid would only take room from the predecessor: a cache write and read of 8,925 tokens took 19.0 us so, 17.0 without.
 // The error is left to cudaGetLastError.
 template <class... P, class... A>
 inline void launch_early(void (*kernel)(P...), int sm_count, uint32_t grid, uint32_t threads, cudaStream_t s, A... args) {

@@ -4,8 +4,8 @@
 // o + d (16 + c).  The hidden 16 makes a code the top mantissa bits of the f16 or bf16 number 16 + c, so the
 // attention kernel builds tensor-core operands from it with one mask-and-or.  The layout of a block of 16 tokens
 // is in include/moestream_cuda.h.  Both kernels are bound by memory: every row and every block byte moves once.
-// Reading 61,000 tokens of 4 heads of 128 dims (154 MB) takes 29 us, 5.3 TB/s; writing and reading back 8,900 tokens
-// of 8 heads of 64 dims 17 us, two launches and their look-ups before the 48 MB.
+// Reading 57,200 tokens of 4 heads of 128 dims (154 MB) takes 29 us, 5.3 TB/s, writing them 46 us, 3.3 TB/s (instructions of
+// the quantiser); writing 8,925 tokens of 8 heads of 64 dims (24 MB) takes 10.7 us, most of it latency, and reading them back 6.5.
 #include <type_traits>
 
 #include "../../include/moestream_cuda.h"
@@ -133,7 +133,7 @@ struct Group8 {
 };
 constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to an integer in the low bits
 // The kernel executes 142 warp instructions for 8 values of each lane; with the values one by one and __fdiv_rn it were 201,
-// which bound it (write and read back 8,900 tokens of 8 heads of 64 dims: 19.0 us for 17.0).
+// which bound it (write and read back 8,925 tokens of 8 heads of 64 dims: 19.0 us for 17.0).
 template <class T>
 __device__ __forceinline__ Group8 quantise8(const Raw8<T>& raw) {
   Group8 g;
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const ms_kv4_cache c
 template <class T, int HD>
 cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_rows& r, bool write, cudaStream_t s) {
   // 16 rows share a look-up, with few rows down to 2, so that a decode step spreads over the SMs (write and read back,
-  // 16 rows against 2: 15.0 / 5.1 us for 32 tokens, 19.5 / 22.3 for 8,900, where the rule takes 8: 17.0)
+  // 16 rows against 2: 15.0 / 5.1 us for 32 tokens, 19.5 / 22.3 for 8,925, where the rule takes 8: 17.0)
   int rows = kRows;
   while (rows > 2 && (int64_t)r.total < (int64_t)rows * 4 * d.sm_count) rows /= 2;
   const uint32_t grid = (uint32_t)(((int64_t)r.total + rows - 1) / rows);

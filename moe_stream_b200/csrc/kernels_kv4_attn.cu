@@ -27,11 +27,11 @@
 // one of 1 lost all of their share).  The maximum is raised only when a lane's probabilities of a tile add up to more than
 // 2^15, 2^8 times the largest: p stays inside f16, and most tiles need no reduction over the lanes.
 //
-// Measured: 32 sequences of 8,300 tokens on average, 4 heads of 128 dims (162 MB): 43 us, 3.7 TB/s; one of 131,072
+// Measured: 32 sequences of 7,845 tokens on average, 4 heads of 128 dims (161 MB): 44 us, 3.7 TB/s; one of 131,072
 // tokens, 8 heads of 64 dims (84 MB, f16): 28 us; one of 4,097 tokens: 9 us.  Bulk copies alone stream the first
-// in 30 us; 3 us go by before the first copy (lengths, split, page numbers), the blocks end up to 4 us apart, and the
-// second kernel takes 3 to 4 us.  The loop issues 330 instructions a warp for 16 tokens of 128 dims and keeps the
-// issue slots half busy.
+// in 30 us, about what the loop takes; 3 us go by before the first copy (lengths, split, page numbers), the blocks end up to
+// 4 us apart, and the second kernel takes 3 to 4 us.  The loop issues 330 instructions a warp for 16 tokens of 128 dims and
+// keeps the issue slots half busy.
 #include <type_traits>
 
 #include "../../include/moestream_cuda.h"
@@ -48,7 +48,7 @@ constexpr int kWarps = 4, kThreads = kWarps * 32, kStages = 2;
 constexpr int kTileBytes = 5120;          // 16 * 20 * 16 for every head_dim
 // blocks of an SM: 3 leave 168 registers a thread; 256 dims, or 16 rows of 128, need more than that.  (4 blocks, with
 // a few values spilled, have more warps but more starts, joins and parts: 47 us for 3's 44 on a batch of 32
-// sequences of 8,300 tokens on average, 4 heads of 128 dims.)
+// sequences of 7,845 tokens on average, 4 heads of 128 dims.)
 __host__ __device__ constexpr int blocks_per_sm(int hd, int nt) { return hd * nt >= 256 ? 2 : 3; }
 constexpr int kMinTiles = kWarps;         // tiles of a range at least: one per warp
 constexpr int kExtra = 8;                 // empty tiles behind those of a job
@@ -777,7 +777,7 @@ cudaError_t start(const DevCtx& d, const ms_kv4_cache& c, const ms_kv4_attn& a, 
   cfg.dynamicSmemBytes = 0;
   // Few jobs have many parts each, and one round of loads costs about a microsecond: 16 loads at a time then.  One
   // sequence, 4 heads of 128 dims, 8 against 16: 7.6 / 7.6 us (200 tokens), 9.1 / 8.7 (4,097), 12.8 / 11.1 (9,000).  With
-  // many jobs the blocks' registers count: 32 sequences of 8,300 tokens on average 43.5 against 45.2 us.
+  // many jobs the blocks' registers count: 32 sequences of 7,845 tokens on average 43.5 against 45.2 us.
   if (ranges_of(d, HD, NT) >= 32 * (int)cfg.gridDim.x)
     return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, HD, NT, 16>, c, a, row_tiles, ranges_of(d, HD, NT));
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, HD, NT, 8>, c, a, row_tiles, ranges_of(d, HD, NT));

@@ -25,10 +25,12 @@
 //
 // CL = 2 (256 dims): two blocks of a cluster share each MMA (M = 256), each with its own 128 rows and half of every K
 // and V tile.  With one query tile a block, 256 dims read K and V from L2 for 128 rows only, 28 bytes a cycle and
-// SM, and waited for them: a chunk of 2,048 queries behind 9,001 keys took 352 us, with pairs 238 us (337 GFLOP,
-// 1,414 TFLOP/s, 84 % of the cuBLAS rate measured on this GPU).  128 dims have two query tiles a block and lose by
-// pairs, whose two blocks wait for each other: 463 us became 526 us for 8,192 tokens of 32 heads (550 GFLOP; now
-// 459 us, 1,198 TFLOP/s, 72 %).  There a key tile takes 3,900 cycles: the chain of scores (512), softmax (1,890, of which
+// SM, and waited for them: a chunk of 2,048 queries behind 9,001 keys (336 GFLOP) took 352 us, with pairs 238 us on the same
+// card, in a graph.  Now 241 us in a graph (1,394 TFLOP/s, 83 % of the cuBLAS rate in a burst) and 284 us call after call, under the
+// power cap (1,186 TFLOP/s, 84 % of cuBLAS's sustained rate); its 128 pairs take two rounds of 74.  128 dims have two query
+// tiles a block and lose by pairs, whose two blocks wait for each other: 463 us became 526 us for 8,192 tokens of 32 heads
+// (550 GFLOP; now 462 to 519 us in a graph by the card's clock, 538 us call after call: 1,023 TFLOP/s, 73 % of the sustained
+// rate).  There a key tile takes 3,900 cycles: the chain of scores (512), softmax (1,890, of which
 // 1,024 are the special-function unit's for 128 exponentials a thread), values (512) and four hand-overs of a
 // slot, two slots in turn.  What did not help there: a quarter of the exponentials as polynomials, probabilities
 // handed over in halves, two threads a row (515 us), an MMA warp for each slot (interleaving their MMAs costs 40 %),
