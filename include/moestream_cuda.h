@@ -281,7 +281,7 @@ MS_API ms_status ms_qk_norm_rope(ms_ctx* ctx, const ms_qk_rope* args);
  * product (f16: besides that rounding a probability may be off by 2^-32 of the row's largest); a query without keys
  * gives zeros.  Rows of out behind cu_q[n_seqs] are left as they were.
  * total_q / total_k: rows of q and out / of k and v (cu_q[n_seqs] and cu_k[n_seqs] at most).  Offsets that descend, are
- * negative or end behind these are reported (MS_ERR_DEVICE_INDEX); out then holds nothing of use for any sequence.
+ * negative or end behind these are reported (MS_ERR_DEVICE_INDEX); which sequences out then holds is open.
  * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 128 per kv head and 65536; strides multiples of
  * 8 elements, pointers 16-byte aligned; out must not overlap the inputs.  The values of v are finite. */
 typedef struct ms_prompt_attn {
